@@ -298,6 +298,113 @@ int soc_op_embedding(soc_ctx* ctx, const int32_t* ids, const void* table, int32_
 /* ElementwiseMulOp::Run: y = a * b elementwise over rows * n. */
 int soc_op_mul(soc_ctx* ctx, const float* a, const float* b, float* y, int32_t rows, int32_t n);
 
+/* ---- serving from a paged key-value cache, on caller device memory. The reference keeps one contiguous cache
+ *      (KVCache, Mac/gpu/include/runtime/kv_cache.h:23-79) and has no counterpart. One layer's cache is a pool of pages
+ *      of page_size positions; a sequence's positions [0, length) lie in the pages its block table row names, in order.
+ *      A step is: soc_paged_plan (pages, slots and positions from the requests' lengths), then in each layer
+ *      soc_paged_append (rotary positions; keys and values into their slots) and soc_paged_attention_decode, and at the
+ *      end soc_logprobs of the chosen tokens. All calls check that each operand lies inside one device allocation of
+ *      the context's device, are queued on the context stream without waiting, and hold their workspace in the context;
+ *      an operand changed, freed or read by other means first waits for them (soc_ctx_synchronize). Operands of one call
+ *      must not overlap except where its comment says so. What device memory holds (lengths, page ids, slots) is checked
+ *      on the device: no value in it makes a kernel leave the operands' bounds. ---- */
+/* Pairs rotated together: half (i, i + rotary_dim / 2), or interleaved (2 i, 2 i + 1). */
+enum { SOC_ROPE_HALF = 0, SOC_ROPE_INTERLEAVED = 1 };
+/* Long contexts: positions divided by `factor`; theta raised by factor^(d / (d - 2)); or the frequencies that turn
+ * fewer than beta_slow times within original_max_position divided by `factor`, those that turn more than beta_fast
+ * times kept, and a ramp between (d = rotary_dim). */
+enum { SOC_ROPE_UNSCALED = 0, SOC_ROPE_LINEAR = 1, SOC_ROPE_NTK = 2, SOC_ROPE_YARN = 3 };
+typedef struct soc_rope_spec {
+  int32_t head_dim;              /* 2 .. 1024, even                                                             */
+  int32_t rotary_dim;            /* the first rotary_dim dims of each head are rotated; even, 2 .. head_dim     */
+  int32_t layout;                /* SOC_ROPE_HALF or SOC_ROPE_INTERLEAVED                                       */
+  int32_t scaling;               /* SOC_ROPE_UNSCALED, _LINEAR, _NTK (rotary_dim > 2) or _YARN                  */
+  double theta;                  /* > 1                                                                         */
+  double factor;                 /* >= 1; ignored when unscaled                                                 */
+  int32_t original_max_position; /* YaRN: > 0                                                                   */
+  double beta_fast, beta_slow;   /* YaRN: 0 and 0 mean 32 and 1; else beta_fast > beta_slow > 0                 */
+  double attention_factor;       /* YaRN: multiplies cosines and sines; 0 means 0.1 ln(factor) + 1; else > 0    */
+} soc_rope_spec;
+typedef struct soc_rope soc_rope;
+/* The frequencies of a spec, kept on the context's device. Destroyed before its context. */
+int soc_rope_create(soc_ctx* ctx, const soc_rope_spec* spec, soc_rope** out);
+int soc_rope_destroy(soc_rope* rope);
+/* Rotates `heads` heads of `rows` rows x -> y (SOC_DTYPE_F32 or _F16; rows x_stride and y_stride elements apart, each at
+ * least heads * head_dim): row r at position positions[r] (device memory, any int32), or position_offset + r where
+ * positions is NULL. The angles are formed in 64 bits. Dims from rotary_dim on are copied. y may be x with the same
+ * stride. */
+int soc_rope_apply(const soc_rope* rope, const void* x, int64_t x_stride, void* y, int64_t y_stride, int32_t dtype,
+                   int32_t rows, int32_t heads, const int32_t* positions, int32_t position_offset);
+/* One layer's pages: fp16; dim i of the position at place t of page p and KV head h is element
+ * p * page_stride + (h * page_size + t) * head_dim + i of `keys` and of `values`. page_stride: 0, or at least
+ * kv_heads * page_size * head_dim and a multiple of 8 (pools that interleave layers, or keys with values). page_size:
+ * 16, 32, 64, 128 or 256; head_dim: 64 or 128; num_pages * page_size < 2^31; keys and values 16-byte aligned. */
+typedef struct soc_paged_cache {
+  void* keys;
+  void* values;
+  int64_t page_stride;
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+} soc_paged_cache;
+/* What a plan found wrong (bits of its status word). */
+enum { SOC_PLAN_LENGTHS = 1, SOC_PLAN_CURSORS = 2, SOC_PLAN_PAGES = 4, SOC_PLAN_ROWS = 8 };
+/* Pages, positions and slots of a step that brings request i from old_lens[i] to new_lens[i] positions, 1 <= n <= 4096
+ * (all pointers: device memory). The free pages are entries head .. tail - 1 of free_ring [num_pages] (modulo its size;
+ * cursors_in = {head, tail}, 64-bit counts that only grow; a new cache has all page ids in the ring and {0, num_pages}).
+ *   longer (prompt, chunk, decoded token): its rows are the positions old .. new - 1, and where they need further pages
+ *     these are taken from the head and written to block_table row i (entries of table_stride elements a row, max_pages
+ *     <= 2^18 of them used), requests in order, pages in order;
+ *   shorter (finished: 0; or rolled back): its table's pages beyond the new length go to the ring's tail, requests in
+ *     order, pages in order; the table row is left as it is.
+ * row_starts [n + 1]: exclusive sums of the rows. positions, slots [max_rows] (max_rows <= 2^22): each row's position
+ * and slot (page * page_size + place; -1 where its page id is none of the cache); rows from the total on get position 0
+ * and slot -1. cursors_out = the cursors after the step (may be cursors_in). Pages given back are first taken by a later
+ * plan. *status = 0; or bits, and then nothing is taken or given: row_starts and positions are 0, slots -1, cursors_out =
+ * cursors_in, table and ring untouched. The bits: LENGTHS, a length is negative or beyond max_pages; CURSORS, the ring
+ * would hold fewer than 0 or more than num_pages entries; PAGES, more pages needed than free; ROWS, more than max_rows
+ * rows. The result does not depend on timing: equal inputs give equal outputs. */
+int soc_paged_plan(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const int32_t* new_lens, int32_t page_size,
+                   int32_t* block_table, int32_t max_pages, int64_t table_stride, int32_t* free_ring, int32_t num_pages,
+                   const int64_t* cursors_in, int64_t* cursors_out, int32_t* row_starts, int32_t* positions,
+                   int32_t* slots, int32_t max_rows, int32_t* status);
+/* A step's new rows into the cache: row r's kv_heads keys, rotated at positions[r], and values go to slots[r], rounded
+ * to fp16 to nearest; its q_heads queries, rotated, to q_out. q, k, v (SOC_DTYPE_F32 or _F16) and q_out (same type):
+ * rows q_stride, k_stride, v_stride, q_out_stride elements apart, so that the three may be parts of one fused
+ * projection; q_out may be q with the same stride. q_heads may be 0 (q and q_out unused). rope: of the cache's head_dim;
+ * NULL stores keys unrotated (then q_heads must be 0 and positions is unused). A row whose slot is negative or outside
+ * the cache is skipped: nothing of it is stored, its q_out row is left as it is. Slots of one call must differ. */
+int soc_paged_append(soc_ctx* ctx, const soc_paged_cache* cache, const soc_rope* rope, const void* q, int64_t q_stride,
+                     const void* k, int64_t k_stride, const void* v, int64_t v_stride, int32_t dtype, void* q_out,
+                     int64_t q_out_stride, int32_t rows, int32_t q_heads, const int32_t* positions,
+                     const int32_t* slots);
+/* Attention of one token of each of n sequences over its cached positions [0, seq_lens[i]) (its own among them): q and
+ * out (SOC_DTYPE_F32 or _F16) [n][q_heads * head_dim], rows q_stride and out_stride elements apart (out may be q with the
+ * same stride); q_heads / kv_heads a whole number up to 16; scores times `scale` (finite; 0 means 1 / sqrt(head_dim)).
+ * block_table: max_pages entries a row used, rows table_stride apart; pages may be shared by sequences. lse (nullable)
+ * [n][q_heads]: log sum exp of the scores, to join with attention over other keys. A sequence of length 0 (or below)
+ * gets zeros and lse -inf; one whose length goes beyond max_pages, or whose table names a page outside the cache within
+ * its length, gets NaN. What lies in its last page behind its length is not used, whatever it holds. A NaN or infinity
+ * among the queries, keys or values used makes what it enters not finite. */
+int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const void* q, int64_t q_stride,
+                               int32_t dtype, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
+                               const int32_t* seq_lens, int32_t n, int32_t q_heads, float scale, void* out,
+                               int64_t out_stride, float* lse);
+/* Log probabilities under softmax(logits / temperature) (temperature <= 0 taken as 1, as in soc_sample_topk) of rows of
+ * `vocab` logits (SOC_DTYPE_F32 or _F16, row_stride elements apart, device memory):
+ *   tokens [rows] (nullable): logprobs[r] = the log probability of token tokens[r]; ranks[r] (nullable) = how many tokens
+ *     stand before it in the order below. A token of -1 stands for none: 0 and -1; another id outside the vocabulary:
+ *     NaN and -1.
+ *   entropy [rows] (nullable), in nats.
+ *   top_ids, top_logprobs [rows][top_n] (0 <= top_n <= min(64, vocab); NULL at 0): the tokens of the largest logits in
+ *     order, equal logits by lowest id.
+ * -inf masks a token: log probability -inf, no part in the entropy. A row of nothing but -inf has log probabilities -inf
+ * and entropy 0. A row that holds a NaN or +inf has log probabilities and entropy NaN; NaNs are ordered above +inf. */
+int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab,
+                 float temperature, const int32_t* tokens, float* logprobs, int32_t* ranks, float* entropy,
+                 int32_t top_n, int32_t* top_ids, float* top_logprobs);
+
 /* ---- seeded synthetic data (this project's generator; the reference has none) ---- */
 int soc_synth_normal_f16(uint64_t seed, const char* name, float sigma, int64_t offset, int64_t n, uint16_t* out);
 int soc_synth_uniform_f16(uint64_t seed, const char* name, float lo, float hi, int64_t offset, int64_t n,

@@ -31,6 +31,21 @@ class QwenConfigC(C.Structure):
     ]
 
 
+class RopeSpecC(C.Structure):
+    _fields_ = [
+        ("head_dim", C.c_int32), ("rotary_dim", C.c_int32), ("layout", C.c_int32), ("scaling", C.c_int32),
+        ("theta", C.c_double), ("factor", C.c_double), ("original_max_position", C.c_int32),
+        ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("attention_factor", C.c_double),
+    ]
+
+
+class PagedCacheC(C.Structure):
+    _fields_ = [
+        ("keys", C.c_void_p), ("values", C.c_void_p), ("page_stride", C.c_int64), ("num_pages", C.c_int32),
+        ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+    ]
+
+
 @dataclass(frozen=True)
 class QwenConfig:
     """Model hyper-parameters (the keys of the bundle's HF config, Mac/cpu/src/qwen3_config.cpp:20-36)."""
@@ -175,6 +190,13 @@ def lib() -> C.CDLL:
         "soc_op_mul": (C.c_int, [P, P, P, P, I32, I32]),
         "soc_qmm": (C.c_int, [P, P, P, I32, P, P, I32, I32, I32]),
         "soc_dequant": (C.c_int, [P, P, I32, P, P, I32, I32]),
+        "soc_rope_create": (C.c_int, [P, C.POINTER(RopeSpecC), C.POINTER(P)]),
+        "soc_rope_destroy": (C.c_int, [P]),
+        "soc_rope_apply": (C.c_int, [P, P, I64, P, I64, I32, I32, I32, P, I32]),
+        "soc_paged_plan": (C.c_int, [P, I32, P, P, I32, P, I32, I64, P, I32, P, P, P, P, P, I32, P]),
+        "soc_paged_append": (C.c_int, [P, P, P, P, I64, P, I64, P, I64, I32, P, I64, I32, I32, P, P]),
+        "soc_paged_attention_decode": (C.c_int, [P, P, P, I64, I32, P, I64, I32, P, I32, I32, F32, P, I64, P]),
+        "soc_logprobs": (C.c_int, [P, P, I32, I64, I32, I32, F32, P, P, P, P, I32, P, P]),
         "soc_synth_normal_f16": (C.c_int, [U64, C.c_char_p, F32, I64, I64, P]),
         "soc_synth_uniform_f16": (C.c_int, [U64, C.c_char_p, F32, F32, I64, I64, P]),
         "soc_synth_tokens": (C.c_int, [U64, C.c_char_p, I32, I64, P]),
@@ -621,3 +643,77 @@ def attention_prefill(ctx: Context, q_dev: int, k_dev: int, v_dev: int, out_dev:
 def attention_decode(ctx: Context, q_dev: int, k_dev: int, v_dev: int, out_dev: int, kv_len: int, nq: int, nkv: int,
                      cap: int) -> None:
     check(lib().soc_attention_decode(ctx.h, q_dev, k_dev, v_dev, out_dev, kv_len, nq, nkv, 128, cap))
+
+
+# ---- serving from a paged key-value cache ------------------------------------------------------------------------
+DTYPES = {"f32": 0, "f16": 1}
+ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+PLAN_LENGTHS, PLAN_CURSORS, PLAN_PAGES, PLAN_ROWS = 1, 2, 4, 8
+
+
+class Rope:
+    """Rotary frequencies on the device (soc_rope_create). Close it before its context."""
+
+    def __init__(self, ctx: Context, head_dim: int, rotary_dim: int | None = None, *, layout: str = "half",
+                 theta: float = 1_000_000.0, scaling: str = "none", factor: float = 1.0,
+                 original_max_position: int = 0, beta_fast: float = 0.0, beta_slow: float = 0.0,
+                 attention_factor: float = 0.0):
+        self.h = None
+        spec = RopeSpecC(head_dim, head_dim if rotary_dim is None else rotary_dim, ROPE_LAYOUTS[layout],
+                         ROPE_SCALINGS[scaling], theta, factor, original_max_position, beta_fast, beta_slow,
+                         attention_factor)
+        h = C.c_void_p()
+        check(lib().soc_rope_create(ctx.h if ctx is not None else None, C.byref(spec), C.byref(h)))
+        self.h, self.head_dim = h, head_dim
+
+    def apply(self, x: int, y: int, dtype: str, rows: int, heads: int, *, positions: int | None = None,
+              offset: int = 0, x_stride: int | None = None, y_stride: int | None = None) -> None:
+        """soc_rope_apply on device addresses; strides in elements, dense rows by default."""
+        width = heads * self.head_dim
+        check(lib().soc_rope_apply(self.h, x, width if x_stride is None else x_stride, y,
+                                   width if y_stride is None else y_stride, DTYPES[dtype], rows, heads, positions,
+                                   offset))
+
+    def close(self) -> None:
+        if self.h:
+            lib().soc_rope_destroy(self.h)
+            self.h = None
+
+
+class PagedCache:
+    """One layer's pages on caller device memory (soc_paged_cache)."""
+
+    def __init__(self, keys: int, values: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int,
+                 page_stride: int = 0):
+        self.c = PagedCacheC(keys, values, page_stride, num_pages, page_size, kv_heads, head_dim)
+        self.ref = C.byref(self.c)
+
+
+def paged_plan(ctx: Context, n: int, old_lens: int, new_lens: int, page_size: int, block_table: int, max_pages: int,
+               table_stride: int, free_ring: int, num_pages: int, cursors_in: int, cursors_out: int, row_starts: int,
+               positions: int, slots: int, max_rows: int, status: int) -> None:
+    check(lib().soc_paged_plan(ctx.h, n, old_lens, new_lens, page_size, block_table, max_pages, table_stride,
+                               free_ring, num_pages, cursors_in, cursors_out, row_starts, positions, slots, max_rows,
+                               status))
+
+
+def paged_append(ctx: Context, cache: PagedCache, rope: "Rope | None", q: int | None, q_stride: int, k: int,
+                 k_stride: int, v: int, v_stride: int, dtype: str, q_out: int | None, q_out_stride: int, rows: int,
+                 q_heads: int, positions: int | None, slots: int) -> None:
+    check(lib().soc_paged_append(ctx.h, cache.ref, rope.h if rope is not None else None, q, q_stride, k, k_stride, v,
+                                 v_stride, DTYPES[dtype], q_out, q_out_stride, rows, q_heads, positions, slots))
+
+
+def paged_attention_decode(ctx: Context, cache: PagedCache, q: int, q_stride: int, dtype: str, block_table: int,
+                           table_stride: int, max_pages: int, seq_lens: int, n: int, q_heads: int, scale: float,
+                           out: int, out_stride: int, lse: int | None = None) -> None:
+    check(lib().soc_paged_attention_decode(ctx.h, cache.ref, q, q_stride, DTYPES[dtype], block_table, table_stride,
+                                           max_pages, seq_lens, n, q_heads, scale, out, out_stride, lse))
+
+
+def logprobs(ctx: Context, logits: int, dtype: str, row_stride: int, rows: int, vocab: int, temperature: float,
+             tokens: int | None, logprobs: int | None, ranks: int | None, entropy: int | None, top_n: int,
+             top_ids: int | None, top_logprobs: int | None) -> None:
+    check(lib().soc_logprobs(ctx.h, logits, DTYPES[dtype], row_stride, rows, vocab, temperature, tokens, logprobs,
+                             ranks, entropy, top_n, top_ids, top_logprobs))

@@ -44,6 +44,12 @@ struct soc_ctx {
   size_t op_part_floats = 0;
   int* op_counters = nullptr;
   size_t op_counter_ints = 0;
+  // paged serving operators (soc_paged_*, soc_logprobs): partial results and arrival counters, grown on demand; every
+  // kernel leaves the counters at zero
+  char* serve_ws = nullptr;
+  size_t serve_ws_bytes = 0;
+  int* serve_counters = nullptr;
+  size_t serve_counter_ints = 0;
   // soc_forward with token ids in device memory: set by the staging kernel when an id lies outside [0, vocab)
   int* id_err = nullptr;
 };
@@ -61,5 +67,31 @@ MemRange classify_range(const void* p, size_t bytes);
 // SOC_OK when every (pointer, bytes) of a caller's device operands lies inside one device allocation (null pointers
 // with 0 bytes pass); otherwise SOC_ERR_INVALID naming the operand. Called before any kernel reads caller memory.
 int check_device_operand(const char* what, const void* p, size_t bytes);
+
+// The same for `rows` rows of `width` elements of `size` bytes, `stride` elements apart (at least width), aligned to an
+// element and on the context's device.
+int check_device_rows(const soc_ctx* ctx, const char* what, const void* p, int64_t rows, int64_t stride, int64_t width,
+                      int size);
+
+// Grows the context's serve_ws to `bytes` and its zeroed serve_counters to `ints`.
+int ensure_serve_ws(soc_ctx* ctx, size_t bytes, size_t ints);
+
+// Makes the context's device current for the calling thread while it lives: streams and allocations belong to it.
+class DeviceScope {
+ public:
+  explicit DeviceScope(const soc_ctx* ctx) {
+    if (hipGetDevice(&before_) != hipSuccess) before_ = ctx->device;
+    if (before_ != ctx->device && hipSetDevice(ctx->device) == hipSuccess) changed_ = true;
+  }
+  ~DeviceScope() {
+    if (changed_) (void)hipSetDevice(before_);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+
+ private:
+  int before_ = 0;
+  bool changed_ = false;
+};
 
 }  // namespace soc

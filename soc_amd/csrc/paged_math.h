@@ -1,0 +1,66 @@
+// paged_math.h - index arithmetic of the paged key-value cache and of its page planner: every index that comes out of
+// caller memory on the device (page ids, slots, ring cursors, lengths) passes one of these before it becomes an address.
+// Plain functions, so that a host program can check them with hostile values.
+#pragma once
+
+#include <stdint.h>
+
+#if defined(__HIPCC__)
+#define SOC_HD __host__ __device__ __forceinline__
+#else
+#define SOC_HD inline
+#endif
+
+namespace soc {
+
+// Pages that hold `len` positions (len >= 0; 0 pages for 0).
+SOC_HD int32_t pages_of(int32_t len, int page_shift) { return len <= 0 ? 0 : ((len - 1) >> page_shift) + 1; }
+
+// A page id as it may be used: itself, or -1 where it names no page of the cache.
+SOC_HD int32_t checked_page(int32_t page, int32_t num_pages) { return page >= 0 && page < num_pages ? page : -1; }
+
+// A slot (page * page_size + place) as it may be used: itself, or -1 where it lies outside the cache.
+SOC_HD int32_t checked_slot(int32_t slot, int32_t num_pages, int page_shift) {
+  return slot >= 0 && (slot >> page_shift) < num_pages ? slot : -1;
+}
+
+// The slot of place `offset` of page `page`; -1 where the page is none of the cache (num_pages << page_shift fits 31
+// bits).
+SOC_HD int32_t slot_of(int32_t page, int32_t offset, int32_t num_pages, int page_shift) {
+  return checked_page(page, num_pages) < 0 ? -1 : (page << page_shift) + offset;
+}
+
+// The keys of a sequence that may be read: its length; 0 for a negative one; -1 for one beyond its table's pages.
+SOC_HD int32_t checked_length(int32_t len, int32_t max_pages, int page_shift) {
+  return len < 0 ? 0 : pages_of(len, page_shift) > max_pages ? -1 : len;
+}
+
+// Place of entry number `cursor` + i of a ring of `size` entries, for any cursor.
+SOC_HD int32_t ring_place(int64_t cursor, int32_t i, int32_t size) {
+  const uint64_t at = static_cast<uint64_t>(cursor) % static_cast<uint64_t>(size) + static_cast<uint32_t>(i);
+  return static_cast<int32_t>(at % static_cast<uint64_t>(size));
+}
+
+// What a step asks for that brings a request from `before` to `after` positions: new rows, pages to take and to give
+// back. The sums over kPlanMaxRequests requests stay within 32 bits: rows and pages saturate beyond kPlanMaxRows, which
+// the plan refuses, and a table row has at most kPlanMaxPages pages.
+constexpr int32_t kPlanMaxRequests = 4096, kPlanMaxRows = 1 << 22, kPlanMaxPages = 1 << 18;
+struct PlanItem {
+  int32_t rows, take, give;
+  bool bad;  // a length that is negative or longer than the table's pages
+};
+SOC_HD PlanItem plan_item(int32_t before, int32_t after, int32_t max_pages, int page_shift) {
+  PlanItem p{0, 0, 0, false};
+  if (before < 0 || after < 0 || pages_of(before, page_shift) > max_pages || pages_of(after, page_shift) > max_pages) {
+    p.bad = true;
+    return p;
+  }
+  const int32_t had = pages_of(before, page_shift), want = pages_of(after, page_shift);
+  const int32_t most = kPlanMaxRows + 1;
+  if (after > before) p.rows = after - before < most ? after - before : most;
+  if (want > had) p.take = want - had;
+  if (had > want) p.give = had - want;
+  return p;
+}
+
+}  // namespace soc
