@@ -385,8 +385,8 @@ int soc_paged_append(soc_ctx* ctx, const soc_paged_cache* cache, const soc_rope*
  * block_table: max_pages entries a row used, rows table_stride apart; pages may be shared by sequences. lse (nullable)
  * [n][q_heads]: log sum exp of the scores, to join with attention over other keys. A sequence of length 0 (or below)
  * gets zeros and lse -inf; one whose length goes beyond max_pages, or whose table names a page outside the cache within
- * its length, gets NaN. What lies in its last page behind its length is not used, whatever it holds. A NaN or infinity
- * among the queries, keys or values used makes what it enters not finite. */
+ * its length, gets NaN. What lies in its last page behind its length is not used, whatever it holds. Where a NaN or an
+ * infinity is among the queries, keys or values used, what it enters is the formula's result or NaN. */
 int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const void* q, int64_t q_stride,
                                int32_t dtype, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
                                const int32_t* seq_lens, int32_t n, int32_t q_heads, float scale, void* out,

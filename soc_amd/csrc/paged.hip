@@ -207,10 +207,25 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 }
 
 // ---- decode attention ------------------------------------------------------------------------------------------------
+// One block per (sequence, KV head, chunk of keys); four waves take the chunk's 32-key tiles in turn, each with the
+// group's query heads, a running maximum m and sum l and the output so far (in base 2: p = 2^(t - m)). The waves join in
+// LDS; of several chunks the last block to finish joins them all, in chunk order.
+//
+// The keys and values are read once, 16 bytes a lane, and are matrix operands as they come from memory:
+//   scores  S [16 keys][16 columns] = K . Q^T, v_mfma_f32_16x16x32_f16: lane l holds 8 dims of key l % 16, and of the
+//           query column l % 16. A column is a query head's fp16 high part or (8 columns on) what fp32 has beyond it, so
+//           high + low gives the score with about 22 bits of the query, at no further matrix work: a group has at most 8
+//           heads (NT = 1), or 16 in two tiles. Queries are scaled by a power of two first, so that high and low are
+//           normal fp16 numbers whatever the queries' magnitude.
+//   output  O^T [16 dims][16 columns] += V^T . P^T: S leaves 4 keys of each half tile in a lane, which are the 8 keys of
+//           the operand P^T; a lane reads 8 dims of those 8 keys (rows of 256 bytes across 16 lanes) and v_perm_b32
+//           turns its 8 x 8 block, one instruction for 4 bytes: no LDS, no lane exchange. P is split high and low over
+//           the columns as the queries are, and scaled by 2^14 so that small weights stay normal fp16 numbers.
+// Keys behind the sequence's end are read as its last key and get weight 0: what memory holds there is never used.
 struct PagedAttnArgs {
   const f16 *keys, *values;
   int64_t page_stride;
-  int num_pages, page_shift, nkv, group, max_pages;
+  int num_pages, page_shift, nkv, group, max_pages, n;
   const void* q;
   int64_t q_stride;
   const int32_t* table;
@@ -220,61 +235,318 @@ struct PagedAttnArgs {
   void* out;
   int64_t out_stride;
   float* lse;
+  int splits, most, grid;  // attention_chunk
+  float* part;             // [n][nkv][grid][group * (HD + 2)]: outputs, then maxima, then sums
+  int* arrived;            // [n][nkv], zero between launches
 };
 
-template <typename T, int HD>
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kWeightBits = 14.0f;  // weights are held times 2^14
+
+// Reduces over the four lanes l % 16 + {0, 16, 32, 48}; every lane gets the result.
+template <typename F>
+__device__ __forceinline__ float across_rows(float x, F f) {
+  const uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t v = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// x of this lane + x of the lane 8 columns on (mod 16): high and low part.
+__device__ __forceinline__ float both_parts(float x) { return x + dpp_mov<0x128>(x); }
+
+template <typename T, int HD, int NT>
 __global__ __launch_bounds__(256) void k_paged_attention(PagedAttnArgs a) {
-  constexpr int E = HD / kWave;
-  __shared__ float ms[4], ls[4], os[4][HD];
-  const int nq = a.nkv * a.group;
-  const int b = blockIdx.x / nq, h = blockIdx.x % nq, g = h / a.group;
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  constexpr int KC = HD / 32;  // 32-dim steps of a score
+  constexpr int VD = HD / 16;  // dims of a value row a lane reads: 8 (16 bytes) or 4
+  constexpr int HEADS = 8 * NT;
+  typedef uint32_t VReg __attribute__((ext_vector_type(VD / 2)));
+  __shared__ float so[4][HEADS][HD], sm[4][HEADS], sl[4][HEADS];
+  __shared__ float weight[256][HEADS], sums[256][HEADS];  // of up to 256 chunks
+  __shared__ int last;
+
+  const int g = blockIdx.x % a.nkv, rest = blockIdx.x / a.nkv;
+  const int b = rest % a.n, s = rest / a.n;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, row = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.group;
+  const float nan = __builtin_nanf("");
+  T* out = static_cast<T*>(a.out) + b * a.out_stride + static_cast<int64_t>(g) * G * HD;
+  float* lse = a.lse != nullptr ? a.lse + (static_cast<int64_t>(b) * a.nkv + g) * G : nullptr;
   const int len = checked_length(a.lens[b], a.max_pages, a.page_shift);
-  const T* q = static_cast<const T*>(a.q) + b * a.q_stride + h * HD + lane * E;
-  float qv[E], o[E];
-  for (int i = 0; i < E; ++i) {
-    qv[i] = static_cast<float>(q[i]) * a.scale;
-    o[i] = 0.0f;
+  if (len <= 0) {
+    if (s != 0) return;
+    for (int i = tid; i < G * HD; i += 256) out[i] = static_cast<T>(len < 0 ? nan : 0.0f);
+    if (lse != nullptr && tid < G) lse[tid] = len < 0 ? nan : -INFINITY;
+    return;
   }
-  float m = -INFINITY, l = 0.0f;
-  bool lost = len < 0;
-  for (int j = wid; j < len; j += 4) {
-    const int page = checked_page(a.table[b * a.table_stride + (j >> a.page_shift)], a.num_pages);
-    if (page < 0) {
-      lost = true;
-      break;
+  const int chunk = attention_chunk(len, a.splits, a.most, a.grid);
+  const int blocks = (len - 1) / chunk + 1;
+  if (s >= blocks) return;
+  const uint32_t c0 = static_cast<uint32_t>(s) * chunk;
+  const int tiles = (min(chunk, len - static_cast<int>(c0)) - 1) / 32 + 1;
+  const int mine = (tiles - wid + 3) / 4;  // this wave's: wid, wid + 4, ..
+  const int32_t* table = a.table + b * a.table_stride;
+  const uint32_t mask = (1u << a.page_shift) - 1;
+  const f16* keys = a.keys + (static_cast<int64_t>(g) << a.page_shift) * HD;
+  const f16* values = a.values + (static_cast<int64_t>(g) << a.page_shift) * HD;
+
+  // keys count in unsigned words: those behind a length next to 2^31 do not wrap below it
+  auto within = [&](uint32_t key) { return min(key, static_cast<uint32_t>(len) - 1); };
+  // lane l holds the page of half tile l % 2 of this wave's tile l / 2 (32 tiles ahead)
+  bool lost = false;
+  auto pages_from = [&](int first) {
+    const uint32_t key = within(c0 + (wid + 4 * (first + (lane >> 1))) * 32 + (lane & 1) * 16);
+    const int page = checked_page(table[key >> a.page_shift], a.num_pages);
+    lost |= page < 0;
+    return max(page, 0);
+  };
+  int pages = pages_from(0);
+
+  u32x4 kr[2][KC];
+  VReg vr[2][4];
+  // tile i of this wave; key and value rows of a half tile are in one page
+  auto load_keys = [&](int i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t page = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + h);
+      const uint32_t key = within(c0 + (wid + 4 * i) * 32 + h * 16 + col);
+      const f16* p = keys + page * a.page_stride + ((key & mask) * HD + row * 8);
+#pragma unroll
+      for (int c = 0; c < KC; ++c) kr[h][c] = load_stream16(p + c * 32);
     }
-    const int64_t at = page * a.page_stride +
-                       ((static_cast<int64_t>(g) << a.page_shift) + (j & ((1 << a.page_shift) - 1))) * HD + lane * E;
-    float s = 0.0f;
-    for (int i = 0; i < E; ++i) s += qv[i] * static_cast<float>(a.keys[at + i]);
-    s = wave_sum(s);
-    const float m1 = fmaxf(m, s), f = m1 == -INFINITY ? 0.0f : expf(m - m1), p = m1 == -INFINITY ? 0.0f : expf(s - m1);
-    l = l * f + p;
-    for (int i = 0; i < E; ++i) o[i] = o[i] * f + p * static_cast<float>(a.values[at + i]);
-    m = m1;
+  };
+  auto load_values = [&](int i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t page = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + h);
+      const f16* base = values + page * a.page_stride;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t key = within(c0 + (wid + 4 * i) * 32 + h * 16 + row * 4 + j);
+        vr[h][j] = __builtin_nontemporal_load(
+            (const __attribute__((address_space(1))) VReg*)(base + ((key & mask) * HD + col * VD)));
+      }
+    }
+  };
+  if (mine > 0) {
+    load_keys(0);
+    load_values(0);
   }
-  if (lost) l = __builtin_nanf("");
-  if (lane == 0) {
-    ms[wid] = m;
-    ls[wid] = l;
+
+  // the query columns
+  f16x8 qb[NT][KC];
+  float to_log2[NT];  // score of the scaled query -> base-2 exponent
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int head = t * 8 + (col & 7);
+    float x[KC][8];
+    float big = 0.0f;
+    const T* q = static_cast<const T*>(a.q) + b * a.q_stride + (static_cast<int64_t>(g) * G + min(head, G - 1)) * HD;
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[c][i] = head < G ? static_cast<float>(q[c * 32 + row * 8 + i]) : 0.0f;
+        big = fmaxf(big, fabsf(x[c][i]));
+      }
+    big = across_rows(big, [](float u, float v) { return fmaxf(u, v); });
+    // the largest becomes 2^13 .. 2^14
+    const int e = big > 0.0f && big < INFINITY ? min(14 - ilogbf(big) - 1, 126) : 0;
+    const float up = ldexpf(1.0f, e);
+    to_log2[t] = ldexpf(a.scale * kLog2e, -e);
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = x[c][i] * up;
+        const f16 high = static_cast<f16>(v);
+        qb[t][c][i] = col < 8 ? high : static_cast<f16>(v - static_cast<float>(high));
+      }
   }
-  for (int i = 0; i < E; ++i) os[wid][lane * E + i] = o[i];
+
+  float m[NT], l[NT];
+  f32x4 o[NT][VD];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < VD; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  for (int i = 0; i < mine; ++i) {
+    const uint32_t key0 = c0 + (wid + 4 * i) * 32;
+    f32x4 sc[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        sc[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+          sc[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16x8(kr[h][c]), qb[t][c], sc[t][h], 0, 0, 0);
+      }
+    const bool more = i + 1 < mine;
+    // pages of the next 32 tiles, before they are needed; the values of tile i are already on their way
+    if (more && ((i + 1) & 31) == 0) pages = pages_from(i + 1);
+    if (more) load_keys(i + 1);
+    f16x8 pb[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float x[8];
+      float top = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float v = both_parts(sc[t][h][r]) * to_log2[t];
+          x[4 * h + r] = key0 + h * 16 + row * 4 + r < static_cast<uint32_t>(len) ? v : -INFINITY;
+          top = fmaxf(top, x[4 * h + r]);
+        }
+      top = fmaxf(m[t], across_rows(top, [](float u, float v) { return fmaxf(u, v); }));
+      const float f = __builtin_amdgcn_exp2f(m[t] - top);
+      if (__ballot(top != m[t]) != 0) {
+#pragma unroll
+        for (int d = 0; d < VD; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[t][d][r] *= f;
+      }
+      m[t] = top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float p = __builtin_amdgcn_exp2f((x[j] - top) + kWeightBits);  // the difference first: scores may be large
+        sum += p;
+        const f16 high = static_cast<f16>(p);
+        pb[t][j] = col < 8 ? high : static_cast<f16>(p - static_cast<float>(high));
+      }
+      l[t] = l[t] * f + sum;
+    }
+#pragma unroll
+    for (int d = 0; d < VD; ++d) {
+      u32x4 av;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)  // keys 2 w and 2 w + 1 of the lane's 8, dim d of its VD
+        av[w] = __builtin_amdgcn_perm(vr[w >> 1][2 * (w & 1) + 1][d >> 1], vr[w >> 1][2 * (w & 1)][d >> 1],
+                                      d & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16x8(av), pb[t], o[t][d], 0, 0, 0);
+    }
+    if (more) load_values(i + 1);
+  }
+
+  // the four waves
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const float sum = across_rows(l[t], [](float u, float v) { return u + v; });
+    if (row == 0 && col < 8) {
+      sm[wid][t * 8 + col] = m[t];
+      sl[wid][t * 8 + col] = sum;
+    }
+#pragma unroll
+    for (int d = 0; d < VD; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = both_parts(o[t][d][r]);
+        if (col < 8) so[wid][t * 8 + col][(row * 4 + r) * VD + d] = v;
+      }
+  }
+  lost = __syncthreads_or(lost);
+  const int64_t pair = static_cast<int64_t>(b) * a.nkv + g;
+  const int stride = G * (HD + 2);
+  float* part = a.part + (pair * a.grid + s) * stride;
+  // wave 0 has a tile, so the maximum is a number (or NaN scores make the sums NaN)
+  auto joined = [&](int h, float* w) {
+    const float top = fmaxf(fmaxf(sm[0][h], sm[1][h]), fmaxf(sm[2][h], sm[3][h]));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w[u] = sl[u][h] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(sm[u][h] - top);
+    return top;
+  };
+  for (int i = tid; i < G * HD; i += 256) {
+    const int h = i / HD, d = i % HD;
+    float w[4];
+    joined(h, w);
+    float x = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      x += w[u] * so[u][h][d];
+      sum += w[u] * sl[u][h];
+    }
+    if (blocks == 1) out[i] = static_cast<T>(lost ? nan : x / sum);
+    else st_dev(part + i, x);
+  }
+  if (tid < G) {
+    float w[4], sum = 0.0f;
+    const float top = joined(tid, w);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sum += w[u] * sl[u][tid];
+    if (lost) sum = nan;
+    if (blocks > 1) {
+      st_dev(part + G * HD + tid, top);
+      st_dev(part + G * HD + G + tid, sum);
+    } else if (lse != nullptr) {
+      lse[tid] = (top + __builtin_amdgcn_logf(sum) - kWeightBits) * kLn2;
+    }
+  }
+  if (blocks == 1) return;
+
+  // the chunks: this block's part is out before its arrival is counted
+  wait_mem();
   __syncthreads();
-  const float top = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
-  float total = 0.0f;
-  for (int w = 0; w < 4; ++w) total += ls[w] != ls[w] || top != -INFINITY ? ls[w] * expf(ms[w] - top) : 0.0f;
-  const bool nan = total != total || ls[0] != ls[0] || ls[1] != ls[1] || ls[2] != ls[2] || ls[3] != ls[3];
-  const int d = threadIdx.x;
-  if (d < HD) {
-    float x = 0.0f;
-    for (int w = 0; w < 4; ++w)
-      if (ls[w] > 0.0f) x += os[w][d] * expf(ms[w] - top);
-    x = nan ? __builtin_nanf("") : total > 0.0f ? x / total : 0.0f;
-    static_cast<T*>(a.out)[b * a.out_stride + h * HD + d] = static_cast<T>(x);
+  if (tid == 0) last = atomicAdd(a.arrived + pair, 1) == blocks - 1;
+  __syncthreads();
+  if (!last) return;
+  const float* all = a.part + pair * a.grid * stride;
+  for (int i = tid; i < blocks * G; i += 256) {
+    const int u = i / G, h = i - u * G;
+    const float* p = all + static_cast<int64_t>(u) * stride + G * HD + h;
+    weight[u][h] = ld_dev(p);
+    sums[u][h] = ld_dev(p + G);
   }
-  if (d == 0 && a.lse != nullptr)
-    a.lse[static_cast<int64_t>(b) * nq + h] = nan ? __builtin_nanf("") : total > 0.0f ? top + logf(total) : -INFINITY;
+  __syncthreads();
+  for (int h = wid; h < G; h += 4) {
+    float top = -INFINITY, sum = 0.0f;
+    for (int u = lane; u < blocks; u += 64) top = fmaxf(top, weight[u][h]);
+    top = wave_max(top);
+    for (int u = lane; u < blocks; u += 64) {
+      const float w = __builtin_amdgcn_exp2f(weight[u][h] - top);
+      weight[u][h] = w;
+      sum += w * sums[u][h];
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) {
+      sl[0][h] = sum;
+      if (lse != nullptr) lse[h] = (top + __builtin_amdgcn_logf(sum) - kWeightBits) * kLn2;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < G * HD; i += 256) {
+    const int h = i / HD;
+    float x = 0.0f;
+    for (int u0 = 0; u0 < blocks; u0 += 8) {  // eight parts on their way at a time, added in order
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = ld_dev(all + static_cast<int64_t>(min(u0 + j, blocks - 1)) * stride + i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (u0 + j < blocks) x += weight[u0 + j][h] * v[j];
+    }
+    out[i] = static_cast<T>(x / sl[0][h]);
+  }
+  if (tid == 0) st_dev(a.arrived + pair, 0);
+}
+
+template <typename T, int HD>
+hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s) {
+  auto* kernel = a.group <= 8 ? k_paged_attention<T, HD, 1> : k_paged_attention<T, HD, 2>;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.n) * a.nkv * a.grid), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+hipError_t launch_paged_attention(const PagedAttnArgs& a, bool f32, int hd, hipStream_t s) {
+  if (hd == 128) return f32 ? launch_paged_attention<float, 128>(a, s) : launch_paged_attention<f16, 128>(a, s);
+  return f32 ? launch_paged_attention<float, 64>(a, s) : launch_paged_attention<f16, 64>(a, s);
 }
 
 int shift_of(int page_size) {
@@ -464,10 +736,25 @@ int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const
   a.out = out;
   a.out_stride = out_stride;
   a.lse = lse;
-  auto* kernel = size == 4 ? (hd == 128 ? soc::k_paged_attention<float, 128> : soc::k_paged_attention<float, 64>)
-                           : (hd == 128 ? soc::k_paged_attention<soc::f16, 128> : soc::k_paged_attention<soc::f16, 64>);
-  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(n) * q_heads), dim3(256), 0, ctx->stream, a);
-  return soc::hip_status(hipGetLastError(), "paged attention");
+  a.n = n;
+  const int64_t pairs = static_cast<int64_t>(n) * cache->kv_heads;
+  if (pairs > INT32_MAX / 256) return soc::fail(SOC_ERR_INVALID, "paged attention: too many sequences times KV heads");
+  // splits of a sequence: enough blocks for the card where there are few sequences, and none longer than `most` keys,
+  // so that ragged lengths even out
+  const int64_t longest = static_cast<int64_t>(max_pages) * cache->page_size;
+  const size_t part = static_cast<size_t>(a.group) * (hd + 2) * sizeof(float);
+  const int64_t room = std::max<int64_t>(1, (int64_t{512} << 20) / static_cast<int64_t>(pairs * part));
+  a.splits = static_cast<int>((1024 + pairs - 1) / pairs);
+  a.most = static_cast<int>(std::max<int64_t>(1024, ((longest + 31) / 32 + 127) / 128 * 128));
+  a.grid = static_cast<int>(std::min({std::max<int64_t>(a.splits, (longest + a.most - 1) / a.most),
+                                      (longest + 127) / 128, room, int64_t{256}}));
+  if (a.grid > 1) {
+    SOC_TRY(soc::ensure_serve_ws(ctx, static_cast<size_t>(pairs) * a.grid * part, static_cast<size_t>(pairs)));
+    a.part = reinterpret_cast<float*>(ctx->serve_ws);
+    a.arrived = ctx->serve_counters;
+  }
+  const hipError_t e = soc::launch_paged_attention(a, size == 4, hd, ctx->stream);
+  return soc::hip_status(e, "paged attention");
   SOC_API_END
 }
 

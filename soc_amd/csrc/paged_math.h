@@ -35,6 +35,16 @@ SOC_HD int32_t checked_length(int32_t len, int32_t max_pages, int page_shift) {
   return len < 0 ? 0 : pages_of(len, page_shift) > max_pages ? -1 : len;
 }
 
+// Keys a block of the decode attention takes of a sequence of `len` > 0 keys: whole tiles of 128 (32 for each of its four
+// waves), so that the sequence gets at least `splits` blocks while it has tiles for them, and no block more than `most`
+// keys; but never more than `grid` blocks.
+SOC_HD int32_t attention_chunk(int32_t len, int32_t splits, int32_t most, int32_t grid) {
+  int32_t want = (len - 1) / most + 1;
+  want = want > splits ? want : splits;
+  want = want < grid ? want : grid;
+  return ((len - 1) / want / 128 + 1) * 128;
+}
+
 // Place of entry number `cursor` + i of a ring of `size` entries, for any cursor.
 SOC_HD int32_t ring_place(int64_t cursor, int32_t i, int32_t size) {
   const uint64_t at = static_cast<uint64_t>(cursor) % static_cast<uint64_t>(size) + static_cast<uint32_t>(i);
