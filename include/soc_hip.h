@@ -392,7 +392,7 @@ int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const
                                const int32_t* seq_lens, int32_t n, int32_t q_heads, float scale, void* out,
                                int64_t out_stride, float* lse);
 /* Log probabilities under softmax(logits / temperature) (temperature <= 0 taken as 1, as in soc_sample_topk) of rows of
- * `vocab` logits (SOC_DTYPE_F32 or _F16, row_stride elements apart, device memory):
+ * `vocab` logits, at most 2^20 (SOC_DTYPE_F32 or _F16, row_stride elements apart, device memory):
  *   tokens [rows] (nullable): logprobs[r] = the log probability of token tokens[r]; ranks[r] (nullable) = how many tokens
  *     stand before it in the order below. A token of -1 stands for none: 0 and -1; another id outside the vocabulary:
  *     NaN and -1.

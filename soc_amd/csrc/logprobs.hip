@@ -4,6 +4,7 @@
 // With M the row's largest logit, d_i = (x_i - M) / temperature, S = sum exp(d_i) and D = sum d_i exp(d_i):
 //   log p_i = d_i - log S,  entropy = log S - D / S.
 // Differences are taken before they are scaled, so that nothing of the logits' common size enters the sums.
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -27,6 +28,10 @@ struct LogprobArgs {
   int top_n;
   int32_t* top_ids;
   float* top_logprobs;
+  int chunks;       // blocks a row
+  struct Part* parts;    // [rows][chunks]
+  uint64_t* tops;        // [rows][chunks][top_n]: each chunk's first tokens, 0 where it has fewer
+  int* arrived;          // [rows], zero between launches
 };
 
 // Order of logits as unsigned words: NaNs first, then by value, both zeros alike; never 0 nor all ones.
@@ -46,88 +51,256 @@ __device__ __forceinline__ uint64_t key_of(float x, int id) {
   return static_cast<uint64_t>(order_of(x)) << 32 | static_cast<uint32_t>(~id);
 }
 
-// Running sums of a part of a row: largest logit, sum of exp(d), sum of d exp(d).
-struct Sums {
+// One block per chunk of a row: 256 threads with E logits each in registers, read once in 16-byte loads. The chunk's
+// maximum comes first, so that every exponential is taken once; the count of tokens before the given one is a ballot per
+// logit. Of the top n, each thread's largest token stands for its E: the n-th largest of those 256 keys is a threshold
+// that at most n threads reach, so at most n E tokens (64 of normal data) are candidates, and those rank each other. No
+// step depends on how many values are equal. The last block of a row to finish joins its chunks, in chunk order.
+constexpr int kThreads = 256;
+constexpr int kMaxKeys = 4096;  // candidates of a chunk (kMaxTop threads of 64 tokens), and keys that one block joins
+
+struct Part {  // of a chunk: largest logit, sum of 2^d, sum of d 2^d (d: base-2 exponent below the largest), rank count
   float m, s, d;
+  int above;
 };
-__device__ __forceinline__ Sums join(Sums a, Sums b, float inv_t) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return Sums{m, 0.0f, 0.0f};
-  Sums r{m, 0.0f, 0.0f};
-  const float ua = (a.m - m) * inv_t, fa = expf(ua);  // a part of -inf alone has f = 0
-  if (fa > 0.0f) {                                     // u may be -inf where f is 0
-    r.s += a.s * fa;
-    r.d += fa * (a.d + ua * a.s);
+
+// The n-th largest of `count` keys in LDS (distinct, or 0 for none), by the calling wave: at least 1; fewer than n keys
+// are not below it. Bisection of the order, then of the ids among equal orders.
+__device__ __forceinline__ uint64_t nth_largest(const uint64_t* keys, int count, int n) {
+  const int lane = threadIdx.x & (kWave - 1);
+  uint64_t t = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const uint64_t tried = t | 1ull << bit;
+    int c = 0;
+    for (int i = lane; i < (count + kWave - 1) / kWave * kWave; i += kWave)
+      c += __popcll(__ballot(i < count && keys[i] >= tried));
+    if (c >= n) t = tried;
+    if (c == n) break;  // exactly the n largest reach it
   }
-  const float ub = (b.m - m) * inv_t, fb = expf(ub);
-  if (fb > 0.0f) {
-    r.s += b.s * fb;
-    r.d += fb * (b.d + ub * b.s);
+  return t > 0 ? t : 1;
+}
+
+template <typename T, int E>
+__global__ __launch_bounds__(kThreads) void k_logprobs(LogprobArgs a) {
+  constexpr int VW = 16 / sizeof(T), NV = E / VW, C = kThreads * E;
+  typedef T Vec __attribute__((ext_vector_type(VW)));
+  __shared__ uint64_t keys[kMaxKeys];
+  __shared__ uint64_t group[kThreads];
+  __shared__ uint64_t first[kMaxTop];
+  __shared__ float red[3][4];
+  __shared__ int count[4];
+  __shared__ uint64_t threshold;
+  __shared__ int found, last;
+
+  const int64_t r = blockIdx.x / a.chunks;
+  const int c = blockIdx.x % a.chunks;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const T* x = static_cast<const T*>(a.logits) + r * a.row_stride;
+  // 16-byte loads start at the aligned address at or before the row, whose first logit is element `skip` of them
+  const int skip = static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+  const int base = c * C - skip + tid * VW;
+
+  const int lo = c * C - skip, hi = lo + C;  // the chunk's ids, some of them outside the row at its ends
+  const bool inner = lo >= 0 && hi <= a.vocab;
+  float v[E];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int i = base + k * kThreads * VW;
+    if (inner || (i >= 0 && i + VW <= a.vocab)) {
+      const Vec u = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(x + i));
+#pragma unroll
+      for (int j = 0; j < VW; ++j) v[k * VW + j] = static_cast<float>(u[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VW; ++j)
+        v[k * VW + j] = i + j >= 0 && i + j < a.vocab ? static_cast<float>(x[i + j]) : -INFINITY;
+    }
   }
-  return r;
+  const int token = a.tokens != nullptr ? a.tokens[r] : -1;
+  const bool given = token >= 0 && token < a.vocab;
+  const float xt = given ? static_cast<float>(x[token]) : 0.0f;
+
+  // largest logit of the thread and where it stands (the lowest place of equal ones)
+  float best = -INFINITY;
+  int at = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (v[e] > best) {
+      best = v[e];
+      at = e;
+    }
+  float m = wave_max(best);
+  if (lane == 0) red[0][wid] = m;
+  if (tid == 0) found = 0;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  // -inf alone sums to 0; NaN, or +inf less itself, makes the sums NaN
+  const float m0 = m == -INFINITY ? 0.0f : m;
+  const float to_log2 = a.inv_t * 1.4426950408889634f;
+  float s = 0.0f, d = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float u = (v[e] - m0) * to_log2;
+    const float p = __builtin_amdgcn_exp2f(u);
+    s += p;
+    d = fmaf(p, fmaxf(u, -1000.0f), d);  // 2^-1000 is 0: a masked logit adds 0, not 0 times -inf
+  }
+  auto place = [&](int e) { return base + (e / VW) * kThreads * VW + e % VW; };  // the id of the thread's logit e
+  // tokens before the given one: equal logits at lower ids, larger ones anywhere. A chunk at the row's ends, one that
+  // holds the token, and a token of NaN take the order key by key (from the cache: registers are not indexed)
+  int above = 0;
+  if (given) {
+    if (inner && hi <= token && xt == xt) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) above += !(v[e] < xt);
+    } else if (inner && lo > token && xt == xt) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) above += !(v[e] <= xt);
+    } else {
+      const uint64_t mine = key_of(xt, token);
+#pragma unroll 4
+      for (int id = max(lo, 0) + tid; id < min(hi, a.vocab); id += kThreads)
+        above += key_of(static_cast<float>(x[id]), id) > mine;
+    }
+  }
+  const float counts = wave_sum(static_cast<float>(above));  // exact: at most 2^20
+  s = wave_sum(s);
+  d = wave_sum(d);
+  if (lane == 0) {
+    red[1][wid] = s;
+    red[2][wid] = d;
+    count[wid] = static_cast<int>(counts);
+  }
+  __syncthreads();
+  s = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  d = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+  above = count[0] + count[1] + count[2] + count[3];
+
+  const int n = a.top_n;
+  if (n > 0) {
+    if (s != s) {  // NaNs stand above all: the thread's largest by order
+      uint64_t key = 0;
+      for (int e = 0; e < E; ++e) {
+        const int id = place(e);
+        if (id >= 0 && id < a.vocab) key = max(key, key_of(static_cast<float>(x[id]), id));
+      }
+      group[tid] = key;
+    } else {
+      // a thread of -inf alone: its first logit that exists
+      if (best == -INFINITY)
+        for (int e = 0; e < E && (place(at) < 0 || place(at) >= a.vocab); ++e) at = e;
+      const int id = place(at);
+      group[tid] = id >= 0 && id < a.vocab ? key_of(best, id) : 0;
+    }
+    __syncthreads();
+    if (wid == 0) {
+      const uint64_t t = nth_largest(group, kThreads, n);
+      if (lane == 0) threshold = t;
+    }
+    if (tid < n) first[tid] = 0;
+    __syncthreads();
+    const uint64_t t = threshold;
+    if (group[tid] >= t) {  // at most n threads: their logits once more, from the cache
+#pragma unroll 4
+      for (int e = 0; e < E; ++e) {
+        const int id = place(e);
+        if (id < 0 || id >= a.vocab) continue;
+        const uint64_t key = key_of(static_cast<float>(x[id]), id);
+        if (key >= t) keys[atomicAdd(&found, 1)] = key;
+      }
+    }
+    __syncthreads();
+    const int candidates = found;
+    for (int i = tid; i < candidates; i += kThreads) {
+      const uint64_t key = keys[i];
+      int rank = 0;
+      for (int j = 0; j < candidates; ++j) rank += keys[j] > key;
+      if (rank < n) first[rank] = key;
+    }
+    __syncthreads();
+  }
+
+  if (a.chunks > 1) {
+    Part* part = a.parts + r * a.chunks;
+    uint64_t* tops = a.tops + r * a.chunks * n;
+    if (tid == 0) {
+      st_dev(&part[c].m, m);
+      st_dev(&part[c].s, s);
+      st_dev(&part[c].d, d);
+      st_dev(&part[c].above, above);
+    }
+    if (tid < n)
+      __hip_atomic_store(tops + c * n + tid, first[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    wait_mem();
+    __syncthreads();
+    if (tid == 0) last = atomicAdd(a.arrived + r, 1) == a.chunks - 1;
+    __syncthreads();
+    if (!last) return;
+    if (tid == 0) st_dev(a.arrived + r, 0);
+    for (int i = tid; i < a.chunks * n; i += kThreads)
+      keys[i] = __hip_atomic_load(tops + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // every wave the same sums
+    m = -INFINITY;
+    for (int u = lane; u < a.chunks; u += kWave) m = fmaxf(m, ld_dev(&part[u].m));
+    m = wave_max(m);
+    s = d = 0.0f;
+    float counted = 0.0f;  // exact: at most 2^20
+    for (int u = lane; u < a.chunks; u += kWave) {
+      const float su = ld_dev(&part[u].s), du = ld_dev(&part[u].d), mu = ld_dev(&part[u].m);
+      const float shift = mu == -INFINITY ? -1000.0f : fmaxf((mu - m) * to_log2, -1000.0f);
+      const float f = __builtin_amdgcn_exp2f(shift);
+      s += su * f;
+      d += f * (du + shift * su);
+      if (su != su) s = su;
+      counted += static_cast<float>(ld_dev(&part[u].above));
+    }
+    s = wave_sum(s);
+    d = wave_sum(d);
+    above = static_cast<int>(wave_sum(counted));
+    if (n > 0) {
+      __syncthreads();
+      if (tid == 0) found = 0;
+      if (wid == 0) {
+        const uint64_t t = nth_largest(keys, a.chunks * n, n);
+        if (lane == 0) threshold = t;
+      }
+      __syncthreads();
+      const uint64_t t = threshold;
+      for (int i = tid; i < a.chunks * n; i += kThreads)
+        if (keys[i] >= t) group[atomicAdd(&found, 1)] = keys[i];  // exactly n: the vocabulary has as many
+      __syncthreads();
+      if (tid < n) {
+        const uint64_t key = group[tid];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += group[j] > key;
+        first[rank] = key;
+      }
+      __syncthreads();
+    }
+  }
+
+  const float nan = __builtin_nanf(""), ln2 = 0.6931471805599453f;
+  const float log_s = s > 0.0f ? __builtin_amdgcn_logf(s) * ln2 : 0.0f;
+  auto log_p = [&](float y) { return s != s ? nan : y == -INFINITY ? -INFINITY : (y - m) * a.inv_t - log_s; };
+  if (tid == 0) {
+    if (a.tokens != nullptr) {
+      a.logprobs[r] = given ? log_p(xt) : token == -1 ? 0.0f : nan;
+      if (a.ranks != nullptr) a.ranks[r] = given ? above : -1;
+    }
+    if (a.entropy != nullptr) a.entropy[r] = s != s ? nan : s > 0.0f ? log_s - d / s * ln2 : 0.0f;
+  }
+  if (tid < n) {
+    const uint64_t key = first[tid];
+    a.top_ids[r * n + tid] = static_cast<int32_t>(~static_cast<uint32_t>(key));
+    a.top_logprobs[r * n + tid] = log_p(value_of(static_cast<uint32_t>(key >> 32)));
+  }
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_logprobs(LogprobArgs a) {
-  __shared__ Sums part[4];
-  __shared__ uint64_t best[4];
-  __shared__ int count[4];
-  const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const T* x = static_cast<const T*>(a.logits) + r * a.row_stride;
-  Sums u{-INFINITY, 0.0f, 0.0f};
-  const int token = a.tokens != nullptr ? a.tokens[r] : -1;
-  const bool given = token >= 0 && token < a.vocab;
-  const uint64_t mine = given ? key_of(static_cast<float>(x[token]), token) : 0;
-  int above = 0;
-  bool bad = false;
-  for (int i = tid; i < a.vocab; i += 256) {
-    const float v = static_cast<float>(x[i]);
-    bad |= !(v < INFINITY);
-    above += key_of(v, i) > mine;
-    u = join(u, Sums{v, v == -INFINITY ? 0.0f : 1.0f, 0.0f}, a.inv_t);
-  }
-  bad = __syncthreads_or(bad);
-  for (int d = 1; d < 64; d <<= 1) {
-    const Sums o{__shfl_xor(u.m, d), __shfl_xor(u.s, d), __shfl_xor(u.d, d)};
-    u = join(u, o, a.inv_t);
-    above += __shfl_xor(above, d);
-  }
-  if (lane == 0) {
-    part[wid] = u;
-    count[wid] = above;
-  }
-  __syncthreads();
-  u = join(join(part[0], part[1], a.inv_t), join(part[2], part[3], a.inv_t), a.inv_t);
-  above = count[0] + count[1] + count[2] + count[3];
-  const float nan = __builtin_nanf("");
-  const float log_s = u.s > 0.0f ? logf(u.s) : 0.0f;
-  auto log_p = [&](float v) { return bad ? nan : v == -INFINITY ? -INFINITY : (v - u.m) * a.inv_t - log_s; };
-  if (tid == 0) {
-    if (a.tokens != nullptr) {
-      a.logprobs[r] = given ? log_p(static_cast<float>(x[token])) : token == -1 ? 0.0f : nan;
-      if (a.ranks != nullptr) a.ranks[r] = given ? above : -1;
-    }
-    if (a.entropy != nullptr) a.entropy[r] = bad ? nan : u.s > 0.0f ? log_s - u.d / u.s : 0.0f;
-  }
-  uint64_t below = ~0ull;
-  for (int k = 0; k < a.top_n; ++k) {
-    uint64_t w = 0;
-    for (int i = tid; i < a.vocab; i += 256) {
-      const uint64_t key = key_of(static_cast<float>(x[i]), i);
-      if (key < below && key > w) w = key;
-    }
-    for (int d = 1; d < 64; d <<= 1) w = max(w, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(w), d)));
-    __syncthreads();
-    if (lane == 0) best[wid] = w;
-    __syncthreads();
-    w = max(max(best[0], best[1]), max(best[2], best[3]));
-    below = w;
-    if (tid == 0) {
-      a.top_ids[r * a.top_n + k] = static_cast<int32_t>(~static_cast<uint32_t>(w));
-      a.top_logprobs[r * a.top_n + k] = log_p(value_of(static_cast<uint32_t>(w >> 32)));
-    }
-  }
+hipError_t launch_logprobs(const LogprobArgs& a, bool small, hipStream_t s) {
+  auto* k = small ? k_logprobs<T, 16> : k_logprobs<T, 64>;
+  hipLaunchKernelGGL(k, dim3(static_cast<uint32_t>(a.rows) * a.chunks), dim3(kThreads), 0, s, a);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -142,8 +315,8 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
   using soc::check_device_rows;
   if (dtype != SOC_DTYPE_F32 && dtype != SOC_DTYPE_F16)
     return soc::fail(SOC_ERR_INVALID, "logprobs: dtype must be F32 or F16");
-  if (rows <= 0 || vocab <= 0 || vocab > (1 << 30))
-    return soc::fail(SOC_ERR_INVALID, "logprobs: need rows > 0 and a vocabulary of 1 to 2^30");
+  if (rows <= 0 || vocab <= 0 || vocab > (1 << 20))
+    return soc::fail(SOC_ERR_INVALID, "logprobs: need rows > 0 and a vocabulary of 1 to 2^20");
   if (top_n < 0 || top_n > soc::kMaxTop || top_n > vocab)
     return soc::fail(SOC_ERR_INVALID, "logprobs: top_n must be 0 to min(64, vocab)");
   if (!std::isfinite(temperature) || (temperature > 0.0f && !std::isfinite(1.0f / temperature)))
@@ -166,12 +339,40 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
     SOC_TRY(check_device_rows(ctx, "logprobs top_ids", top_ids, rows, top_n, top_n, 4));
     SOC_TRY(check_device_rows(ctx, "logprobs top_logprobs", top_logprobs, rows, top_n, top_n, 4));
   }
-  soc::LogprobArgs a{logits, row_stride, rows,    vocab, temperature <= 0.0f ? 1.0f : 1.0f / temperature,
-                     tokens, logprobs,   ranks,   entropy, top_n, top_ids, top_logprobs};
-  auto* kernel = size == 4 ? soc::k_logprobs<float> : soc::k_logprobs<soc::f16>;
-  hipLaunchKernelGGL(kernel, dim3(rows), dim3(256), 0, ctx->stream, a);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? SOC_OK : soc::fail(SOC_ERR_HIP, std::string("logprobs: ") + hipGetErrorString(e));
+  // chunks of 16384 logits; of 4096 where few rows would leave most of the card idle
+  auto chunks_of = [&](int logits_each) { return (vocab + 16 / size - 1 + logits_each - 1) / logits_each; };
+  const bool small = static_cast<int64_t>(rows) * chunks_of(16384) < 1024 &&
+                     chunks_of(4096) * std::max(1, top_n) <= soc::kMaxKeys;
+  const int chunks = chunks_of(small ? 4096 : 16384);
+  const size_t per_row = chunks > 1 ? chunks * (sizeof(soc::Part) + static_cast<size_t>(top_n) * 8) : 0;
+  // rows a launch: its workspace stays below 256 MiB, its grid below 2^31 blocks
+  const int64_t most = std::min<int64_t>(std::max<int64_t>(1, (int64_t{256} << 20) / std::max<size_t>(1, per_row)),
+                                         (int64_t{1} << 30) / chunks);
+  const int step = static_cast<int>(std::min<int64_t>(rows, most));
+  if (chunks > 1) SOC_TRY(soc::ensure_serve_ws(ctx, step * per_row, step));
+  soc::LogprobArgs a{};
+  a.row_stride = row_stride;
+  a.vocab = vocab;
+  a.inv_t = temperature <= 0.0f ? 1.0f : 1.0f / temperature;
+  a.top_n = top_n;
+  a.chunks = chunks;
+  a.tops = reinterpret_cast<uint64_t*>(ctx->serve_ws);
+  a.parts = reinterpret_cast<soc::Part*>(ctx->serve_ws + static_cast<size_t>(step) * chunks * top_n * 8);
+  a.arrived = ctx->serve_counters;
+  for (int64_t r = 0; r < rows; r += step) {
+    a.logits = static_cast<const char*>(logits) + r * row_stride * size;
+    a.rows = static_cast<int>(std::min<int64_t>(step, rows - r));
+    a.tokens = tokens != nullptr ? tokens + r : nullptr;
+    a.logprobs = logprobs != nullptr ? logprobs + r : nullptr;
+    a.ranks = ranks != nullptr ? ranks + r : nullptr;
+    a.entropy = entropy != nullptr ? entropy + r : nullptr;
+    a.top_ids = top_n > 0 ? top_ids + r * top_n : nullptr;
+    a.top_logprobs = top_n > 0 ? top_logprobs + r * top_n : nullptr;
+    const hipError_t e = size == 4 ? soc::launch_logprobs<float>(a, small, ctx->stream)
+                                   : soc::launch_logprobs<soc::f16>(a, small, ctx->stream);
+    if (e != hipSuccess) return soc::fail(SOC_ERR_HIP, std::string("logprobs: ") + hipGetErrorString(e));
+  }
+  return SOC_OK;
   SOC_API_END
 }
 

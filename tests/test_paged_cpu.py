@@ -148,7 +148,7 @@ def test_attention_refusals():
 
 # ---- log probabilities -----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kw,text", [
-    ({"dtype": 2}, "dtype"), ({"rows": 0}, "rows"), ({"vocab": 0}, "vocabulary"), ({"vocab": (1 << 30) + 1}, "vocabulary"),
+    ({"dtype": 2}, "dtype"), ({"rows": 0}, "rows"), ({"vocab": 0}, "vocabulary"), ({"vocab": (1 << 20) + 1}, "vocabulary"),
     ({"top": -1}, "top_n"), ({"top": 65}, "top_n"), ({"vocab": 5, "top": 6}, "top_n"),
     ({"t": float("nan")}, "temperature"), ({"t": float("inf")}, "temperature"), ({"t": 1e-40}, "temperature"),
     ({"tokens": None}, "need tokens"), ({"tokens": None, "logprobs": None}, "nothing"),
