@@ -34,21 +34,30 @@ struct LogprobArgs {
   int* arrived;          // [rows], zero between launches
 };
 
-// Order of logits as unsigned words: NaNs first, then by value, both zeros alike; never 0 nor all ones.
-constexpr uint32_t kOrderNan = 0xffff0000u;  // above +inf's 0xff800000
+// Order of logits as unsigned words: NaNs first, then by value, both zeros alike; never 0 nor all ones. A 16-bit logit's
+// order is in the upper half.
+constexpr uint32_t kOrderNan = 0xffff0000u;  // above +inf's 0xff800000 (16 bits: 0xfc000000)
+template <typename T>
 __device__ __forceinline__ uint32_t order_of(float x) {
   if (x != x) return kOrderNan;
-  const uint32_t b = __float_as_uint(x + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  uint32_t b = __float_as_uint(x + 0.0f);
+  if constexpr (sizeof(T) == 2) b = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<f16>(x + 0.0f))) << 16;
+  const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
+  return sizeof(T) == 2 ? o & 0xffff0000u : o;
 }
+template <typename T>
 __device__ __forceinline__ float value_of(uint32_t o) {
   if (o == kOrderNan) return __builtin_nanf("");
-  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+  const uint32_t b = o & 0x80000000u ? o & 0x7fffffffu : ~o;
+  if constexpr (sizeof(T) == 2) return static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(b >> 16)));
+  return __uint_as_float(b);
 }
-// Order of tokens: by logit, then by lowest id. Distinct for every token of a row; 0 is below all of them,
-// all ones above.
+// Order of tokens: by logit, then by lowest id. Distinct for every token of a row; 0 is below all of them.
+constexpr int kMaxVocab = 1 << 20;
+__device__ __forceinline__ uint32_t low_of(int id) { return static_cast<uint32_t>(kMaxVocab - id); }  // 1 .. 2^20
+template <typename T>
 __device__ __forceinline__ uint64_t key_of(float x, int id) {
-  return static_cast<uint64_t>(order_of(x)) << 32 | static_cast<uint32_t>(~id);
+  return static_cast<uint64_t>(order_of<T>(x)) << 32 | low_of(id);
 }
 
 // One block per chunk of a row: 256 threads with E logits each in registers, read once in 16-byte loads. The chunk's
@@ -57,40 +66,107 @@ __device__ __forceinline__ uint64_t key_of(float x, int id) {
 // that at most n threads reach, so at most n E tokens (64 of normal data) are candidates, and those rank each other. No
 // step depends on how many values are equal. The last block of a row to finish joins its chunks, in chunk order.
 constexpr int kThreads = 256;
-constexpr int kMaxKeys = 4096;  // candidates of a chunk (kMaxTop threads of 64 tokens), and keys that one block joins
+// Keys in LDS: the candidates of a chunk (top_n threads of E tokens); then the top_n of every chunk that one block joins,
+// and those of them at the threshold.
+__host__ __device__ constexpr int key_room(int top_n, int each, int chunks) {
+  return top_n * (each > 2 * chunks ? each : 2 * chunks);
+}
 
 struct Part {  // of a chunk: largest logit, sum of 2^d, sum of d 2^d (d: base-2 exponent below the largest), rank count
   float m, s, d;
   int above;
 };
 
-// The n-th largest of `count` keys in LDS (distinct, or 0 for none), by the calling wave: at least 1; fewer than n keys
-// are not below it. Bisection of the order, then of the ids among equal orders.
-__device__ __forceinline__ uint64_t nth_largest(const uint64_t* keys, int count, int n) {
-  const int lane = threadIdx.x & (kWave - 1);
-  uint64_t t = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const uint64_t tried = t | 1ull << bit;
-    int c = 0;
-    for (int i = lane; i < (count + kWave - 1) / kWave * kWave; i += kWave)
-      c += __popcll(__ballot(i < count && keys[i] >= tried));
-    if (c >= n) t = tried;
-    if (c == n) break;  // exactly the n largest reach it
+// How many of the wave's words, K a lane, are not below x.
+template <int K>
+__device__ __forceinline__ int reaching(const uint32_t (&w)[K], uint32_t x) {
+  int c = 0;
+#pragma unroll
+  for (int j = 0; j < K; ++j) c += __popcll(__ballot(w[j] >= x));
+  return c;
+}
+// Largest and smallest word of the wave (DPP within rows of 16, then the four rows).
+template <typename F>
+__device__ __forceinline__ uint32_t wave_fold(uint32_t v, F f) {
+  v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xB1, 0xF, 0xF, true)));
+  v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4E, 0xF, 0xF, true)));
+  v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x141, 0xF, 0xF, true)));
+  v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x140, 0xF, 0xF, true)));
+  const auto row = [&](int lane) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane)); };
+  return __builtin_amdgcn_readfirstlane(f(f(row(0), row(16)), f(row(32), row(48))));
+}
+// The largest x with bits from `low` up that at least n <= 64 K of the wave's words reach (0 where fewer are above 0), by
+// bisection with ballots from the first bit in which the words differ. Ends as soon as exactly n reach it: *exact. That
+// is after about ten bits of the orders of ordinary logits.
+template <int K>
+__device__ __forceinline__ uint32_t nth_word(const uint32_t (&w)[K], int n, int low, bool* exact) {
+  uint32_t most = w[0], least = w[0];
+#pragma unroll
+  for (int j = 1; j < K; ++j) {
+    most = max(most, w[j]);
+    least = min(least, w[j]);
   }
-  return t > 0 ? t : 1;
+  most = wave_fold(most, [](uint32_t x, uint32_t y) { return max(x, y); });
+  least = wave_fold(least, [](uint32_t x, uint32_t y) { return min(x, y); });
+  const uint32_t differ = most ^ least;
+  const int top = differ == 0 ? -1 : 31 - __builtin_clz(differ);
+  // the bits that all words share: 64 bits, so that the shift by 32 is one
+  uint32_t t = most & static_cast<uint32_t>(~0ull << (top + 1));
+  *exact = false;
+  for (int bit = top; bit >= low; --bit) {
+    const uint32_t x = t | 1u << bit;
+    const int c = reaching(w, x);
+    if (c >= n) t = x;
+    if (c == n) {
+      *exact = true;
+      break;
+    }
+  }
+  return t;
+}
+// The n-th largest of `count` <= 64 K keys (distinct, or 0 for none), by the calling wave: at least 1; where there are
+// fewer than n keys, none is below it. First the orders, then the ids among equal orders.
+template <typename T, int K, typename Key>
+__device__ __forceinline__ uint64_t nth_largest(Key key, int count, int n) {
+  constexpr int kLow = sizeof(T) == 2 ? 16 : 0;
+  const int lane = threadIdx.x & (kWave - 1);
+  uint32_t w[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j)
+    w[j] = j * kWave + lane < count ? static_cast<uint32_t>(key(j * kWave + lane) >> 32) : 0;
+  bool exact;
+  const uint32_t t = nth_word(w, n, kLow, &exact);
+  if (exact) return static_cast<uint64_t>(t) << 32;
+  if (t == 0) return 1;
+  const int ties = n - reaching(w, t + 1);  // wanted of those of order t
+#pragma unroll
+  for (int j = 0; j < K; ++j) w[j] = w[j] == t ? static_cast<uint32_t>(key(j * kWave + lane)) : 0;
+  return static_cast<uint64_t>(t) << 32 | nth_word(w, ties, 0, &exact);
+}
+
+// The n largest of `count` distinct keys in LDS, in order, to `first`, by all threads: each key counts the larger ones.
+__device__ __forceinline__ void rank_first(const uint64_t* keys, int count, int n, uint64_t* first) {
+  for (int i = threadIdx.x; i < count; i += kThreads) {
+    const uint64_t key = keys[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < count; ++j) rank += keys[j] > key;
+    if (rank < n) first[rank] = key;
+  }
 }
 
 template <typename T, int E>
 __global__ __launch_bounds__(kThreads) void k_logprobs(LogprobArgs a) {
   constexpr int VW = 16 / sizeof(T), NV = E / VW, C = kThreads * E;
+  constexpr int kLow = sizeof(T) == 2 ? 16 : 0;  // lowest bit of an order
   typedef T Vec __attribute__((ext_vector_type(VW)));
-  __shared__ uint64_t keys[kMaxKeys];
+  extern __shared__ uint64_t keys[];  // key_room(top_n, E, chunks)
   __shared__ uint64_t group[kThreads];
   __shared__ uint64_t first[kMaxTop];
   __shared__ float red[3][4];
   __shared__ int count[4];
   __shared__ uint64_t threshold;
-  __shared__ int found, last;
+  __shared__ int found, last, tied;
 
   const int64_t r = blockIdx.x / a.chunks;
   const int c = blockIdx.x % a.chunks;
@@ -120,15 +196,9 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LogprobArgs a) {
   const bool given = token >= 0 && token < a.vocab;
   const float xt = given ? static_cast<float>(x[token]) : 0.0f;
 
-  // largest logit of the thread and where it stands (the lowest place of equal ones)
-  float best = -INFINITY;
-  int at = 0;
+  float best = v[0];
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (v[e] > best) {
-      best = v[e];
-      at = e;
-    }
+  for (int e = 1; e < E; ++e) best = fmaxf(best, v[e]);
   float m = wave_max(best);
   if (lane == 0) red[0][wid] = m;
   if (tid == 0) found = 0;
@@ -157,10 +227,10 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LogprobArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) above += !(v[e] <= xt);
     } else {
-      const uint64_t mine = key_of(xt, token);
+      const uint64_t mine = key_of<T>(xt, token);
 #pragma unroll 4
       for (int id = max(lo, 0) + tid; id < min(hi, a.vocab); id += kThreads)
-        above += key_of(static_cast<float>(x[id]), id) > mine;
+        above += key_of<T>(static_cast<float>(x[id]), id) > mine;
     }
   }
   const float counts = wave_sum(static_cast<float>(above));  // exact: at most 2^20
@@ -178,45 +248,65 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LogprobArgs a) {
 
   const int n = a.top_n;
   if (n > 0) {
-    if (s != s) {  // NaNs stand above all: the thread's largest by order
-      uint64_t key = 0;
-      for (int e = 0; e < E; ++e) {
-        const int id = place(e);
-        if (id >= 0 && id < a.vocab) key = max(key, key_of(static_cast<float>(x[id]), id));
+    // the order of the thread's largest; 0 where it has no logit (the lowest of its ids is place(0), or 0). Where the sum
+    // is NaN, a NaN may hide from `best`
+    uint32_t order = place(0) < a.vocab ? order_of<T>(best) : 0;
+    if (s != s) {
+      order = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (place(e) >= 0 && place(e) < a.vocab) order = max(order, order_of<T>(v[e]));
+    }
+    group[tid] = static_cast<uint64_t>(order) << 32;
+    __syncthreads();
+    uint32_t w[kThreads / kWave];  // wave 0
+    if (wid == 0) {
+#pragma unroll
+      for (int j = 0; j < kThreads / kWave; ++j) w[j] = static_cast<uint32_t>(group[j * kWave + lane] >> 32);
+      bool exact;
+      const uint32_t o = nth_word(w, n, kLow, &exact);
+      if (lane == 0) {
+        threshold = static_cast<uint64_t>(o) << 32;
+        tied = !exact && o != 0;
       }
-      group[tid] = key;
-    } else {
-      // a thread of -inf alone: its first logit that exists
-      if (best == -INFINITY)
-        for (int e = 0; e < E && (place(at) < 0 || place(at) >= a.vocab); ++e) at = e;
-      const int id = place(at);
-      group[tid] = id >= 0 && id < a.vocab ? key_of(best, id) : 0;
     }
     __syncthreads();
-    if (wid == 0) {
-      const uint64_t t = nth_largest(group, kThreads, n);
-      if (lane == 0) threshold = t;
+    if (tied) {  // threads whose largest are equal at the threshold: those of the lowest ids
+      const uint32_t o = static_cast<uint32_t>(threshold >> 32);
+      if (order == o) {
+        const float ov = value_of<T>(o);
+        int id = 0;
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e)
+          if ((v[e] == ov || (v[e] != v[e] && ov != ov)) && place(e) >= 0 && place(e) < a.vocab) id = place(e);
+        group[tid] |= low_of(id);
+      }
+      __syncthreads();
+      if (wid == 0) {
+        const int ties = n - reaching(w, o + 1);
+#pragma unroll
+        for (int j = 0; j < kThreads / kWave; ++j)
+          w[j] = w[j] == o ? static_cast<uint32_t>(group[j * kWave + lane]) : 0;
+        bool exact;
+        const uint32_t low = nth_word(w, ties, 0, &exact);
+        if (lane == 0) threshold |= low;
+      }
     }
     if (tid < n) first[tid] = 0;
     __syncthreads();
-    const uint64_t t = threshold;
-    if (group[tid] >= t) {  // at most n threads: their logits once more, from the cache
-#pragma unroll 4
-      for (int e = 0; e < E; ++e) {
-        const int id = place(e);
-        if (id < 0 || id >= a.vocab) continue;
-        const uint64_t key = key_of(static_cast<float>(x[id]), id);
-        if (key >= t) keys[atomicAdd(&found, 1)] = key;
-      }
+    const uint64_t t = max(threshold, uint64_t{1});
+    if (group[tid] >= t) {  // at most n threads
+      const float tv = value_of<T>(static_cast<uint32_t>(t >> 32));
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (!(v[e] < tv)) {
+          const int id = place(e);
+          const uint64_t key = key_of<T>(v[e], id);
+          if (id >= 0 && id < a.vocab && key >= t) keys[atomicAdd(&found, 1)] = key;
+        }
     }
     __syncthreads();
-    const int candidates = found;
-    for (int i = tid; i < candidates; i += kThreads) {
-      const uint64_t key = keys[i];
-      int rank = 0;
-      for (int j = 0; j < candidates; ++j) rank += keys[j] > key;
-      if (rank < n) first[rank] = key;
-    }
+    rank_first(keys, found, n, first);
     __syncthreads();
   }
 
@@ -258,23 +348,23 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LogprobArgs a) {
     d = wave_sum(d);
     above = static_cast<int>(wave_sum(counted));
     if (n > 0) {
+      // the first few of each chunk give a threshold that at least n of all keys reach, and seldom many more
+      const int all = a.chunks * n, few = min(n, (n - 1) / a.chunks + 2);  // chunks * few <= 64 + 2 * 65 words
+      uint64_t* left = keys + all;
       __syncthreads();
       if (tid == 0) found = 0;
       if (wid == 0) {
-        const uint64_t t = nth_largest(keys, a.chunks * n, n);
+        const auto key = [&](int i) { return keys[i / few * n + i % few]; };
+        const uint64_t t = a.chunks * few <= kWave ? nth_largest<T, 1>(key, a.chunks * few, n)
+                                                   : nth_largest<T, 4>(key, a.chunks * few, n);
         if (lane == 0) threshold = t;
       }
       __syncthreads();
       const uint64_t t = threshold;
-      for (int i = tid; i < a.chunks * n; i += kThreads)
-        if (keys[i] >= t) group[atomicAdd(&found, 1)] = keys[i];  // exactly n: the vocabulary has as many
+      for (int i = tid; i < all; i += kThreads)
+        if (keys[i] >= t) left[atomicAdd(&found, 1)] = keys[i];
       __syncthreads();
-      if (tid < n) {
-        const uint64_t key = group[tid];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += group[j] > key;
-        first[rank] = key;
-      }
+      rank_first(left, found, n, first);
       __syncthreads();
     }
   }
@@ -291,16 +381,20 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LogprobArgs a) {
   }
   if (tid < n) {
     const uint64_t key = first[tid];
-    a.top_ids[r * n + tid] = static_cast<int32_t>(~static_cast<uint32_t>(key));
-    a.top_logprobs[r * n + tid] = log_p(value_of(static_cast<uint32_t>(key >> 32)));
+    a.top_ids[r * n + tid] = kMaxVocab - static_cast<int32_t>(static_cast<uint32_t>(key));
+    a.top_logprobs[r * n + tid] = log_p(value_of<T>(static_cast<uint32_t>(key >> 32)));
   }
 }
 
-template <typename T>
-hipError_t launch_logprobs(const LogprobArgs& a, bool small, hipStream_t s) {
-  auto* k = small ? k_logprobs<T, 16> : k_logprobs<T, 64>;
-  hipLaunchKernelGGL(k, dim3(static_cast<uint32_t>(a.rows) * a.chunks), dim3(kThreads), 0, s, a);
+template <typename T, int E>
+hipError_t launch_chunks(const LogprobArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((k_logprobs<T, E>), dim3(static_cast<uint32_t>(a.rows) * a.chunks), dim3(kThreads),
+                     key_room(a.top_n, E, a.chunks) * sizeof(uint64_t), s, a);
   return hipGetLastError();
+}
+template <typename T>
+hipError_t launch_logprobs(const LogprobArgs& a, int each, hipStream_t s) {
+  return each == 16 ? launch_chunks<T, 16>(a, s) : launch_chunks<T, 64>(a, s);
 }
 
 }  // namespace
@@ -315,7 +409,7 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
   using soc::check_device_rows;
   if (dtype != SOC_DTYPE_F32 && dtype != SOC_DTYPE_F16)
     return soc::fail(SOC_ERR_INVALID, "logprobs: dtype must be F32 or F16");
-  if (rows <= 0 || vocab <= 0 || vocab > (1 << 20))
+  if (rows <= 0 || vocab <= 0 || vocab > soc::kMaxVocab)
     return soc::fail(SOC_ERR_INVALID, "logprobs: need rows > 0 and a vocabulary of 1 to 2^20");
   if (top_n < 0 || top_n > soc::kMaxTop || top_n > vocab)
     return soc::fail(SOC_ERR_INVALID, "logprobs: top_n must be 0 to min(64, vocab)");
@@ -340,10 +434,11 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
     SOC_TRY(check_device_rows(ctx, "logprobs top_logprobs", top_logprobs, rows, top_n, top_n, 4));
   }
   // chunks of 16384 logits; of 4096 where few rows would leave most of the card idle
-  auto chunks_of = [&](int logits_each) { return (vocab + 16 / size - 1 + logits_each - 1) / logits_each; };
-  const bool small = static_cast<int64_t>(rows) * chunks_of(16384) < 1024 &&
-                     chunks_of(4096) * std::max(1, top_n) <= soc::kMaxKeys;
-  const int chunks = chunks_of(small ? 4096 : 16384);
+  const bool aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && row_stride * size % 16 == 0;
+  const int skip = aligned ? 0 : 16 / size - 1;  // the most that a row's chunks start before it
+  auto chunks_of = [&](int each) { return (vocab + skip + 256 * each - 1) / (256 * each); };
+  const int each = vocab > (1 << 18) || static_cast<int64_t>(rows) * chunks_of(64) >= 256 ? 64 : 16;
+  const int chunks = chunks_of(each);
   const size_t per_row = chunks > 1 ? chunks * (sizeof(soc::Part) + static_cast<size_t>(top_n) * 8) : 0;
   // rows a launch: its workspace stays below 256 MiB, its grid below 2^31 blocks
   const int64_t most = std::min<int64_t>(std::max<int64_t>(1, (int64_t{256} << 20) / std::max<size_t>(1, per_row)),
@@ -368,8 +463,8 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
     a.entropy = entropy != nullptr ? entropy + r : nullptr;
     a.top_ids = top_n > 0 ? top_ids + r * top_n : nullptr;
     a.top_logprobs = top_n > 0 ? top_logprobs + r * top_n : nullptr;
-    const hipError_t e = size == 4 ? soc::launch_logprobs<float>(a, small, ctx->stream)
-                                   : soc::launch_logprobs<soc::f16>(a, small, ctx->stream);
+    const hipError_t e = size == 4 ? soc::launch_logprobs<float>(a, each, ctx->stream)
+                                   : soc::launch_logprobs<soc::f16>(a, each, ctx->stream);
     if (e != hipSuccess) return soc::fail(SOC_ERR_HIP, std::string("logprobs: ") + hipGetErrorString(e));
   }
   return SOC_OK;
