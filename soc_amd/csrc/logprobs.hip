@@ -60,11 +60,15 @@ __device__ __forceinline__ uint64_t key_of(float x, int id) {
   return static_cast<uint64_t>(order_of<T>(x)) << 32 | low_of(id);
 }
 
-// One block per chunk of a row: 256 threads with E logits each in registers, read once in 16-byte loads. The chunk's
+// One block per chunk of a row: 256 threads with E logits each in registers, read once in 16-byte loads, all requested
+// before the first is used. The chunk's
 // maximum comes first, so that every exponential is taken once; the count of tokens before the given one is a ballot per
 // logit. Of the top n, each thread's largest token stands for its E: the n-th largest of those 256 keys is a threshold
 // that at most n threads reach, so at most n E tokens (64 of normal data) are candidates, and those rank each other. No
 // step depends on how many values are equal. The last block of a row to finish joins its chunks, in chunk order.
+// 777 rows of 151936 fp32 logits with top 8 take 99 us (4.75 TB/s, the rate of a large copy); one row 11.7 us with top
+// 20 and 5.1 us without: there the chain of reading, reducing, selecting, handing over and joining counts. At 32 fp32
+// logits a thread, 64 registers (8 waves a SIMD) are worth 5 % on many rows; in 16 bits they would spill.
 constexpr int kThreads = 256;
 // Keys in LDS: the candidates of a chunk (top_n threads of E tokens); then the top_n of every chunk that one block joins,
 // and those of them at the threshold.
@@ -156,7 +160,7 @@ __device__ __forceinline__ void rank_first(const uint64_t* keys, int count, int 
 }
 
 template <typename T, int E>
-__global__ __launch_bounds__(kThreads) void k_logprobs(LogprobArgs a) {
+__global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k_logprobs(LogprobArgs a) {
   constexpr int VW = 16 / sizeof(T), NV = E / VW, C = kThreads * E;
   constexpr int kLow = sizeof(T) == 2 ? 16 : 0;  // lowest bit of an order
   typedef T Vec __attribute__((ext_vector_type(VW)));
@@ -178,24 +182,37 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LogprobArgs a) {
 
   const int lo = c * C - skip, hi = lo + C;  // the chunk's ids, some of them outside the row at its ends
   const bool inner = lo >= 0 && hi <= a.vocab;
-  float v[E];
+  // all loads are requested before any is used; what lies outside the row is -inf
+  Vec raw[NV];
+  if (inner) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int i = base + k * kThreads * VW;
-    if (inner || (i >= 0 && i + VW <= a.vocab)) {
-      const Vec u = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(x + i));
+    for (int k = 0; k < NV; ++k)
+      raw[k] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(x + base + k * kThreads * VW));
+  } else {
 #pragma unroll
-      for (int j = 0; j < VW; ++j) v[k * VW + j] = static_cast<float>(u[j]);
-    } else {
+    for (int k = 0; k < NV; ++k) {
+      const int i = base + k * kThreads * VW;
 #pragma unroll
-      for (int j = 0; j < VW; ++j)
-        v[k * VW + j] = i + j >= 0 && i + j < a.vocab ? static_cast<float>(x[i + j]) : -INFINITY;
+      for (int j = 0; j < VW; ++j) raw[k][j] = static_cast<T>(-INFINITY);
+      if (i >= 0 && i + VW <= a.vocab) raw[k] = *reinterpret_cast<const Vec*>(x + i);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = base + k * kThreads * VW;
+      if (i < a.vocab && i + VW > 0 && (i < 0 || i + VW > a.vocab)) {  // a vector across the row's first or last id
+#pragma unroll
+        for (int j = 0; j < VW; ++j)
+          if (i + j >= 0 && i + j < a.vocab) raw[k][j] = x[i + j];
+      }
     }
   }
   const int token = a.tokens != nullptr ? a.tokens[r] : -1;
   const bool given = token >= 0 && token < a.vocab;
   const float xt = given ? static_cast<float>(x[token]) : 0.0f;
 
+  float v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = static_cast<float>(raw[e / VW][e % VW]);
   float best = v[0];
 #pragma unroll
   for (int e = 1; e < E; ++e) best = fmaxf(best, v[e]);
@@ -216,21 +233,25 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LogprobArgs a) {
     d = fmaf(p, fmaxf(u, -1000.0f), d);  // 2^-1000 is 0: a masked logit adds 0, not 0 times -inf
   }
   auto place = [&](int e) { return base + (e / VW) * kThreads * VW + e % VW; };  // the id of the thread's logit e
-  // tokens before the given one: equal logits at lower ids, larger ones anywhere. A chunk at the row's ends, one that
-  // holds the token, and a token of NaN take the order key by key (from the cache: registers are not indexed)
+  // tokens before the given one: equal logits at lower ids, larger ones anywhere. What is not of the row is -inf here,
+  // which is never counted: ids below 0 are taken as large ones
   int above = 0;
   if (given) {
-    if (inner && hi <= token && xt == xt) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) above += !(v[e] < xt);
-    } else if (inner && lo > token && xt == xt) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) above += !(v[e] <= xt);
-    } else {
+    if (xt != xt) {  // the NaNs before it: key by key, from the cache
       const uint64_t mine = key_of<T>(xt, token);
 #pragma unroll 4
       for (int id = max(lo, 0) + tid; id < min(hi, a.vocab); id += kThreads)
         above += key_of<T>(static_cast<float>(x[id]), id) > mine;
+    } else if (lo > token) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) above += !(v[e] <= xt);
+    } else if (lo >= 0 && hi <= token) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) above += !(v[e] < xt);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        above += static_cast<uint32_t>(place(e)) < static_cast<uint32_t>(token) ? !(v[e] < xt) : !(v[e] <= xt);
     }
   }
   const float counts = wave_sum(static_cast<float>(above));  // exact: at most 2^20
@@ -349,7 +370,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LogprobArgs a) {
     above = static_cast<int>(wave_sum(counted));
     if (n > 0) {
       // the first few of each chunk give a threshold that at least n of all keys reach, and seldom many more
-      const int all = a.chunks * n, few = min(n, (n - 1) / a.chunks + 2);  // chunks * few <= 64 + 2 * 65 words
+      const int all = a.chunks * n, few = min(n, (n - 1) / a.chunks + 2);  // at most 64 + 2 * 65 words
       uint64_t* left = keys + all;
       __syncthreads();
       if (tid == 0) found = 0;
@@ -394,7 +415,7 @@ hipError_t launch_chunks(const LogprobArgs& a, hipStream_t s) {
 }
 template <typename T>
 hipError_t launch_logprobs(const LogprobArgs& a, int each, hipStream_t s) {
-  return each == 16 ? launch_chunks<T, 16>(a, s) : launch_chunks<T, 64>(a, s);
+  return each == 32 ? launch_chunks<T, 32>(a, s) : launch_chunks<T, 64>(a, s);
 }
 
 }  // namespace
@@ -433,11 +454,12 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
     SOC_TRY(check_device_rows(ctx, "logprobs top_ids", top_ids, rows, top_n, top_n, 4));
     SOC_TRY(check_device_rows(ctx, "logprobs top_logprobs", top_logprobs, rows, top_n, top_n, 4));
   }
-  // chunks of 16384 logits; of 4096 where few rows would leave most of the card idle
   const bool aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && row_stride * size % 16 == 0;
   const int skip = aligned ? 0 : 16 / size - 1;  // the most that a row's chunks start before it
-  auto chunks_of = [&](int each) { return (vocab + skip + 256 * each - 1) / (256 * each); };
-  const int each = vocab > (1 << 18) || static_cast<int64_t>(rows) * chunks_of(64) >= 256 ? 64 : 16;
+  auto chunks_of = [&](int each) { return (vocab + skip + soc::kThreads * each - 1) / (soc::kThreads * each); };
+  // chunks of 8192 logits (chunks of 16384: 777 rows of 151936 top 8 106 -> 94 us, 16 rows 13.3 -> 12.6); of 16384 where
+  // a row is one of them then, without a join (200 rows of 16384 top 5 11.8 -> 9.8 us), and beyond 2^18, for fewer joins
+  const int each = (chunks_of(64) == 1 && chunks_of(32) > 1) || vocab > (1 << 18) ? 64 : 32;
   const int chunks = chunks_of(each);
   const size_t per_row = chunks > 1 ? chunks * (sizeof(soc::Part) + static_cast<size_t>(top_n) * 8) : 0;
   // rows a launch: its workspace stays below 256 MiB, its grid below 2^31 blocks

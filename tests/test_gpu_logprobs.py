@@ -112,6 +112,17 @@ def test_rows_of_the_full_vocabulary(gpu_ctx, rows, top):
     verify(got[0][keep], 0.7, tokens[keep], top, *(g[keep] for g in got[1:]))
 
 
+@pytest.mark.parametrize("vocab", [8192, 8193, 16384, 16385, 2 ** 18, 2 ** 18 + 1, 2 ** 20 - 1, 2 ** 20])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_vocabularies_at_the_chunks_borders(gpu_ctx, vocab, pad):
+    rng = np.random.default_rng(vocab)
+    x = rng.integers(-40, 41, (3, vocab)).astype(np.float32) / 4
+    tokens = np.array([0, vocab - 1, vocab // 2], np.int32)
+    for dtype in ("f32", "f16"):
+        got = run(gpu_ctx, x, dtype, 1.0, tokens, 64, pad)
+        verify(got[0], 1.0, tokens, 64, *got[1:])
+
+
 @pytest.mark.parametrize("t", [0.0, -2.0, 0.05, 0.6, 5.0, 1000.0])
 def test_temperatures(gpu_ctx, t):
     rng = np.random.default_rng(5)
