@@ -222,6 +222,10 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 //           turns its 8 x 8 block, one instruction for 4 bytes: no LDS, no lane exchange. P is split high and low over
 //           the columns as the queries are, and scaled by 2^14 so that small weights stay normal fp16 numbers.
 // Keys behind the sequence's end are read as its last key and get weight 0: what memory holds there is never used.
+//
+// Bound by memory: 200 sequences up to 8192 keys (3.4 GB) 561 us, 6.06 TB/s (a large copy: 4.8); 48 up to 1500 (147 MB)
+// 39.6 us; one of 4071 keys 12.9 us, where launch, length, pages, keys, hand-over and join follow one another.
+// 3 waves a SIMD (168 registers) of 16 KB on their way each; at 2 the last case took 15.3, the second 48.
 struct PagedAttnArgs {
   const f16 *keys, *values;
   int64_t page_stride;
@@ -235,6 +239,7 @@ struct PagedAttnArgs {
   void* out;
   int64_t out_stride;
   float* lse;
+  bool wide_q;             // query rows are 32-byte aligned (16 in fp16): eight values a load
   int splits, most, grid;  // attention_chunk
   float* part;             // [n][nkv][grid][group * (HD + 2)]: outputs, then maxima, then sums
   int* arrived;            // [n][nkv], zero between launches
@@ -256,7 +261,7 @@ __device__ __forceinline__ float across_rows(float x, F f) {
 __device__ __forceinline__ float both_parts(float x) { return x + dpp_mov<0x128>(x); }
 
 template <typename T, int HD, int NT>
-__global__ __launch_bounds__(256) void k_paged_attention(PagedAttnArgs a) {
+__global__ __launch_bounds__(256, HD == 64 ? 4 : NT == 1 ? 3 : 2) void k_paged_attention(PagedAttnArgs a) {
   constexpr int KC = HD / 32;  // 32-dim steps of a score
   constexpr int VD = HD / 16;  // dims of a value row a lane reads: 8 (16 bytes) or 4
   constexpr int HEADS = 8 * NT;
@@ -272,6 +277,28 @@ __global__ __launch_bounds__(256) void k_paged_attention(PagedAttnArgs a) {
   const int G = a.group;
   const float nan = __builtin_nanf("");
   T* out = static_cast<T*>(a.out) + b * a.out_stride + static_cast<int64_t>(g) * G * HD;
+  // a row's first block requests its queries before it knows the length; others may have no keys
+  T qr[NT][KC][8];
+  auto load_queries = [&] {
+    const T* q = static_cast<const T*>(a.q) + b * a.q_stride + static_cast<int64_t>(g) * G * HD + row * 8;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const T* p = q + min(t * 8 + (col & 7), G - 1) * HD;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        if (a.wide_q) {
+          typedef T Q8 __attribute__((ext_vector_type(8)));
+          const Q8 v = *reinterpret_cast<const Q8*>(p + c * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) qr[t][c][i] = v[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) qr[t][c][i] = p[c * 32 + i];
+        }
+      }
+    }
+  };
+  if (s == 0) load_queries();
   float* lse = a.lse != nullptr ? a.lse + (static_cast<int64_t>(b) * a.nkv + g) * G : nullptr;
   const int len = checked_length(a.lens[b], a.max_pages, a.page_shift);
   if (len <= 0) {
@@ -283,6 +310,7 @@ __global__ __launch_bounds__(256) void k_paged_attention(PagedAttnArgs a) {
   const int chunk = attention_chunk(len, a.splits, a.most, a.grid);
   const int blocks = (len - 1) / chunk + 1;
   if (s >= blocks) return;
+  if (s != 0) load_queries();
   const uint32_t c0 = static_cast<uint32_t>(s) * chunk;
   const int tiles = (min(chunk, len - static_cast<int>(c0)) - 1) / 32 + 1;
   const int mine = (tiles - wid + 3) / 4;  // this wave's: wid, wid + 4, ..
@@ -339,27 +367,25 @@ __global__ __launch_bounds__(256) void k_paged_attention(PagedAttnArgs a) {
   float to_log2[NT];  // score of the scaled query -> base-2 exponent
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int head = t * 8 + (col & 7);
-    float x[KC][8];
+    const bool there = t * 8 + (col & 7) < G;
     float big = 0.0f;
-    const T* q = static_cast<const T*>(a.q) + b * a.q_stride + (static_cast<int64_t>(g) * G + min(head, G - 1)) * HD;
 #pragma unroll
     for (int c = 0; c < KC; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[c][i] = head < G ? static_cast<float>(q[c * 32 + row * 8 + i]) : 0.0f;
-        big = fmaxf(big, fabsf(x[c][i]));
+        if (!there) qr[t][c][i] = static_cast<T>(0.0f);
+        big = fmaxf(big, fabsf(static_cast<float>(qr[t][c][i])));
       }
     big = across_rows(big, [](float u, float v) { return fmaxf(u, v); });
     // the largest becomes 2^13 .. 2^14
-    const int e = big > 0.0f && big < INFINITY ? min(14 - ilogbf(big) - 1, 126) : 0;
+    const int e = big > 0.0f && big < INFINITY ? min(13 - ilogbf(big), 126) : 0;
     const float up = ldexpf(1.0f, e);
     to_log2[t] = ldexpf(a.scale * kLog2e, -e);
 #pragma unroll
     for (int c = 0; c < KC; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float v = x[c][i] * up;
+        const float v = static_cast<float>(qr[t][c][i]) * up;
         const f16 high = static_cast<f16>(v);
         qb[t][c][i] = col < 8 ? high : static_cast<f16>(v - static_cast<float>(high));
       }
@@ -498,7 +524,7 @@ __global__ __launch_bounds__(256) void k_paged_attention(PagedAttnArgs a) {
   if (tid == 0) last = atomicAdd(a.arrived + pair, 1) == blocks - 1;
   __syncthreads();
   if (!last) return;
-  const float* all = a.part + pair * a.grid * stride;
+  float* all = a.part + pair * a.grid * stride;
   for (int i = tid; i < blocks * G; i += 256) {
     const int u = i / G, h = i - u * G;
     const float* p = all + static_cast<int64_t>(u) * stride + G * HD + h;
@@ -522,18 +548,25 @@ __global__ __launch_bounds__(256) void k_paged_attention(PagedAttnArgs a) {
     }
   }
   __syncthreads();
-  for (int i = tid; i < G * HD; i += 256) {
-    const int h = i / HD;
-    float x = 0.0f;
-    for (int u0 = 0; u0 < blocks; u0 += 8) {  // eight parts on their way at a time, added in order
-      float v[8];
+  for (int i = tid; i < G * HD / 2; i += 256) {
+    const int h = 2 * i / HD;
+    float x0 = 0.0f, x1 = 0.0f;
+    for (int u0 = 0; u0 < blocks; u0 += 16) {  // sixteen parts on their way at a time, added in order
+      uint64_t v[16];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = ld_dev(all + static_cast<int64_t>(min(u0 + j, blocks - 1)) * stride + i);
+      for (int j = 0; j < 16; ++j)
+        v[j] = __hip_atomic_load(reinterpret_cast<uint64_t*>(all + static_cast<int64_t>(min(u0 + j, blocks - 1)) * stride) + i,
+                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (u0 + j < blocks) x += weight[u0 + j][h] * v[j];
+      for (int j = 0; j < 16; ++j)
+        if (u0 + j < blocks) {
+          const float w = weight[u0 + j][h];
+          x0 += w * __uint_as_float(static_cast<uint32_t>(v[j]));
+          x1 += w * __uint_as_float(static_cast<uint32_t>(v[j] >> 32));
+        }
     }
-    out[i] = static_cast<T>(x / sl[0][h]);
+    out[2 * i] = static_cast<T>(x0 / sl[0][h]);
+    out[2 * i + 1] = static_cast<T>(x1 / sl[0][h]);
   }
   if (tid == 0) st_dev(a.arrived + pair, 0);
 }
@@ -736,18 +769,22 @@ int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const
   a.out = out;
   a.out_stride = out_stride;
   a.lse = lse;
+  a.wide_q = reinterpret_cast<uintptr_t>(q) % (8 * size) == 0 && q_stride % 8 == 0;
   a.n = n;
   const int64_t pairs = static_cast<int64_t>(n) * cache->kv_heads;
   if (pairs > INT32_MAX / 256) return soc::fail(SOC_ERR_INVALID, "paged attention: too many sequences times KV heads");
-  // splits of a sequence: enough blocks for the card where there are few sequences, and none longer than `most` keys,
-  // so that ragged lengths even out
   const int64_t longest = static_cast<int64_t>(max_pages) * cache->page_size;
   const size_t part = static_cast<size_t>(a.group) * (hd + 2) * sizeof(float);
   const int64_t room = std::max<int64_t>(1, (int64_t{512} << 20) / static_cast<int64_t>(pairs * part));
-  a.splits = static_cast<int>((1024 + pairs - 1) / pairs);
-  a.most = static_cast<int>(std::max<int64_t>(1024, ((longest + 31) / 32 + 127) / 128 * 128));
+  // Blocks of a sequence. `splits`: one for each CU where there are few sequences (8 x 1000 keys, 16 query and 8 KV
+  // heads: 12.5 us so, 15.4 with half of them; 8 x 4000, 32 and 8: 27 us, 31 with twice and 34 with four times as many),
+  // but 32 at most (one of 16000 keys, 14 and 2 heads: 19 us with 32 parts a head, 29 with 128). `most`: no block takes
+  // more than 1024 keys, so that ragged lengths even out. `grid`: what is launched for each row of the table, by its
+  // width alone; a large batch has 8 (64 rows of 200 keys in a table 32768 wide: 12 us, 41 with 32, most of them empty).
+  a.splits = static_cast<int>(std::min<int64_t>(32, (256 + pairs - 1) / pairs));
+  a.most = 1024;
   a.grid = static_cast<int>(std::min({std::max<int64_t>(a.splits, (longest + a.most - 1) / a.most),
-                                      (longest + 127) / 128, room, int64_t{256}}));
+                                      std::max<int64_t>(8, 4096 / pairs), (longest + 127) / 128, room, int64_t{256}}));
   if (a.grid > 1) {
     SOC_TRY(soc::ensure_serve_ws(ctx, static_cast<size_t>(pairs) * a.grid * part, static_cast<size_t>(pairs)));
     a.part = reinterpret_cast<float*>(ctx->serve_ws);
