@@ -68,10 +68,24 @@ MemRange classify_range(const void* p, size_t bytes);
 // with 0 bytes pass); otherwise SOC_ERR_INVALID naming the operand. Called before any kernel reads caller memory.
 int check_device_operand(const char* what, const void* p, size_t bytes);
 
-// The same for `rows` rows of `width` elements of `size` bytes, `stride` elements apart (at least width), aligned to an
-// element and on the context's device.
-int check_device_rows(const soc_ctx* ctx, const char* what, const void* p, int64_t rows, int64_t stride, int64_t width,
-                      int size);
+// The operands of one call in device memory: each checked to lie inside one allocation of the context's device. What the
+// runtime answers about an allocation serves the call's further operands in it.
+class Operands {
+ public:
+  explicit Operands(const soc_ctx* ctx) : ctx_(ctx) {}
+  // `rows` rows of `width` elements of `size` bytes, `stride` elements apart (at least width), aligned to an element.
+  int rows(const char* what, const void* p, int64_t rows, int64_t stride, int64_t width, int size);
+  // `count` elements of `size` bytes
+  int array(const char* what, const void* p, int64_t count, int size) { return rows(what, p, 1, count, count, size); }
+
+ private:
+  struct Range {
+    const char *begin, *end;
+  };
+  const soc_ctx* ctx_;
+  Range known_[8];
+  int count_ = 0;
+};
 
 // Grows the context's serve_ws to `bytes` and its zeroed serve_counters to `ints`.
 int ensure_serve_ws(soc_ctx* ctx, size_t bytes, size_t ints);

@@ -427,7 +427,6 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
                  float temperature, const int32_t* tokens, float* logprobs, int32_t* ranks, float* entropy,
                  int32_t top_n, int32_t* top_ids, float* top_logprobs) {
   SOC_API_BEGIN
-  using soc::check_device_rows;
   if (dtype != SOC_DTYPE_F32 && dtype != SOC_DTYPE_F16)
     return soc::fail(SOC_ERR_INVALID, "logprobs: dtype must be F32 or F16");
   if (rows <= 0 || vocab <= 0 || vocab > soc::kMaxVocab)
@@ -442,17 +441,18 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
     return soc::fail(SOC_ERR_INVALID, "logprobs: nothing asked for");
   if (ctx == nullptr) return soc::fail(SOC_ERR_INVALID, "null context");
   soc::DeviceScope device(ctx);
+  soc::Operands operands(ctx);
   const int size = dtype == SOC_DTYPE_F32 ? 4 : 2;
-  SOC_TRY(check_device_rows(ctx, "logprobs logits", logits, rows, row_stride, vocab, size));
+  SOC_TRY(operands.rows("logprobs logits", logits, rows, row_stride, vocab, size));
   if (tokens != nullptr) {
-    SOC_TRY(check_device_rows(ctx, "logprobs tokens", tokens, rows, 1, 1, 4));
-    SOC_TRY(check_device_rows(ctx, "logprobs output", logprobs, rows, 1, 1, 4));
-    if (ranks != nullptr) SOC_TRY(check_device_rows(ctx, "logprobs ranks", ranks, rows, 1, 1, 4));
+    SOC_TRY(operands.array("logprobs tokens", tokens, rows, 4));
+    SOC_TRY(operands.array("logprobs output", logprobs, rows, 4));
+    if (ranks != nullptr) SOC_TRY(operands.array("logprobs ranks", ranks, rows, 4));
   }
-  if (entropy != nullptr) SOC_TRY(check_device_rows(ctx, "logprobs entropy", entropy, rows, 1, 1, 4));
+  if (entropy != nullptr) SOC_TRY(operands.array("logprobs entropy", entropy, rows, 4));
   if (top_n > 0) {
-    SOC_TRY(check_device_rows(ctx, "logprobs top_ids", top_ids, rows, top_n, top_n, 4));
-    SOC_TRY(check_device_rows(ctx, "logprobs top_logprobs", top_logprobs, rows, top_n, top_n, 4));
+    SOC_TRY(operands.rows("logprobs top_ids", top_ids, rows, top_n, top_n, 4));
+    SOC_TRY(operands.rows("logprobs top_logprobs", top_logprobs, rows, top_n, top_n, 4));
   }
   const bool aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && row_stride * size % 16 == 0;
   const int skip = aligned ? 0 : 16 / size - 1;  // the most that a row's chunks start before it
@@ -462,9 +462,9 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
   const int each = (chunks_of(64) == 1 && chunks_of(32) > 1) || vocab > (1 << 18) ? 64 : 32;
   const int chunks = chunks_of(each);
   const size_t per_row = chunks > 1 ? chunks * (sizeof(soc::Part) + static_cast<size_t>(top_n) * 8) : 0;
-  // rows a launch: its workspace stays below 256 MiB, its grid below 2^31 blocks
+  // rows a launch: its workspace stays below 256 MiB, its work-items below 2^32
   const int64_t most = std::min<int64_t>(std::max<int64_t>(1, (int64_t{256} << 20) / std::max<size_t>(1, per_row)),
-                                         (int64_t{1} << 30) / chunks);
+                                         (int64_t{1} << 23) / chunks);
   const int step = static_cast<int>(std::min<int64_t>(rows, most));
   if (chunks > 1) SOC_TRY(soc::ensure_serve_ws(ctx, step * per_row, step));
   soc::LogprobArgs a{};

@@ -15,7 +15,9 @@ namespace {
 // ---- plan ------------------------------------------------------------------------------------------------------------
 // One launch. Every block forms the same exclusive sums over the requests (rows, pages taken, pages given back) in LDS,
 // so that no block waits for another, and then finds the request of each of its rows and pages by bisection. The sums
-// are over at most 4096 lengths, read from L2; a second launch for them alone would cost more than repeating them.
+// are over at most 4096 lengths, read from L2; a second launch for them alone would cost more than repeating them. Bound
+// by latency (lengths, scan, bisection, table, store): 64 requests of one row 5.7 us a call, 4.2 of them the kernel's;
+// 1000 requests with 32768 rows 7.0, 6.9.
 constexpr int kPlanThreads = 256;
 
 struct PlanArgs {
@@ -45,24 +47,43 @@ __device__ __forceinline__ int request_of(const int32_t* starts, int n, int32_t 
   return lo;
 }
 
+// kEach: requests a thread holds in registers, so that all lengths are requested at once.
+template <int kEach>
 __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PlanArgs a) {
-  __shared__ int32_t rows[kPlanMaxRequests + 1], take[kPlanMaxRequests + 1], give[kPlanMaxRequests + 1];
+  constexpr int kRoom = kEach * kPlanThreads;
+  __shared__ int32_t rows[kRoom + 1], take[kRoom + 1], give[kRoom + 1];
+  __shared__ int32_t had[kRoom];  // positions before the step
   __shared__ int32_t wave_total[3][kPlanThreads / kWave];
-  __shared__ int any_bad;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
-  if (tid == 0) any_bad = 0;
   const int64_t head = a.cursors_in[0], tail = a.cursors_in[1];
-  // thread t sums requests [t * per, (t + 1) * per) one after the other, then the block scans the threads' sums
-  const int per = (a.n + kPlanThreads - 1) / kPlanThreads;
-  const int first = min(tid * per, a.n), last = min(first + per, a.n);
+  const int32_t head0 = ring_place(head, a.num_pages), tail0 = ring_place(tail, a.num_pages);
+  // thread t holds requests [t * kEach, (t + 1) * kEach); the block scans the threads' sums
+  const int first = tid * kEach;
+  PlanItem item[kEach];
+  {
+    int32_t before[kEach], after[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      before[j] = after[j] = 0;
+      if (first + j < a.n) {
+        before[j] = a.before[first + j];
+        after[j] = a.after[first + j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      item[j] = plan_item(before[j], after[j], a.max_pages, a.page_shift);
+      if (first + j < a.n) had[first + j] = before[j];
+    }
+  }
   int32_t sum[3] = {0, 0, 0};
   bool bad = false;
-  for (int i = first; i < last; ++i) {
-    const PlanItem p = plan_item(a.before[i], a.after[i], a.max_pages, a.page_shift);
-    bad |= p.bad;
-    sum[0] = min(sum[0] + p.rows, kPlanMaxRows + 1);
-    sum[1] += p.take;
-    sum[2] += p.give;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    bad |= item[j].bad;
+    sum[0] = min(sum[0] + item[j].rows, kPlanMaxRows + 1);
+    sum[1] += item[j].take;
+    sum[2] += item[j].give;
   }
   int32_t incl[3] = {sum[0], sum[1], sum[2]};
 #pragma unroll
@@ -73,12 +94,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PlanArgs a) {
       if (lane >= d) incl[j] += o;
     }
   }
-  __syncthreads();  // any_bad is cleared
-  if (bad) any_bad = 1;
   if (lane == kWave - 1)
 #pragma unroll
     for (int j = 0; j < 3; ++j) wave_total[j][wid] = incl[j];
-  __syncthreads();
+  const bool any_bad = __syncthreads_or(bad) != 0;
   int32_t at[3], total[3];
 #pragma unroll
   for (int j = 0; j < 3; ++j) {
@@ -90,15 +109,16 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PlanArgs a) {
       total[j] += wave_total[j][w];
     }
   }
-  for (int i = first; i < last; ++i) {
-    const PlanItem p = plan_item(a.before[i], a.after[i], a.max_pages, a.page_shift);
-    rows[i] = at[0];
-    take[i] = at[1];
-    give[i] = at[2];
-    at[0] += p.rows;
-    at[1] += p.take;
-    at[2] += p.give;
-  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (first + j < a.n) {
+      rows[first + j] = at[0];
+      take[first + j] = at[1];
+      give[first + j] = at[2];
+      at[0] += item[j].rows;
+      at[1] += item[j].take;
+      at[2] += item[j].give;
+    }
   if (tid == 0) {
     rows[a.n] = total[0];
     take[a.n] = total[1];
@@ -119,11 +139,11 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PlanArgs a) {
     int position = 0, slot = -1;
     if (r < live_rows) {
       const int i = request_of(rows, a.n, static_cast<int32_t>(r));
-      const int before = a.before[i], had = pages_of(before, a.page_shift);
+      const int before = had[i], held = pages_of(before, a.page_shift);
       position = before + (static_cast<int>(r) - rows[i]);
       const int index = position >> a.page_shift;
-      const int page = index < had ? a.table[i * a.table_stride + index]
-                                   : a.ring[ring_place(head, take[i] + (index - had), a.num_pages)];
+      const int page = index < held ? a.table[i * a.table_stride + index]
+                                    : a.ring[ring_place(head0, take[i] + (index - held), a.num_pages)];
       slot = slot_of(page, position & ((1 << a.page_shift) - 1), a.num_pages, a.page_shift);
     }
     a.positions[r] = position;
@@ -135,23 +155,25 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PlanArgs a) {
     // writes, and the ring's places from the tail on are not among those taken from the head (at most num_pages free)
     for (int64_t j = gid; j < total[1]; j += stride) {
       const int i = request_of(take, a.n, static_cast<int32_t>(j));
-      const int had = pages_of(a.before[i], a.page_shift);
-      a.table[i * a.table_stride + had + (j - take[i])] =
-          a.ring[ring_place(head, static_cast<int32_t>(j), a.num_pages)];
+      const int held = pages_of(had[i], a.page_shift);
+      a.table[i * a.table_stride + held + (j - take[i])] =
+          a.ring[ring_place(head0, static_cast<int32_t>(j), a.num_pages)];
     }
     for (int64_t j = gid; j < total[2]; j += stride) {
       const int i = request_of(give, a.n, static_cast<int32_t>(j));
-      const int keep = pages_of(a.after[i], a.page_shift);
-      a.ring[ring_place(tail, static_cast<int32_t>(j), a.num_pages)] =
+      const int keep = pages_of(had[i], a.page_shift) - (give[i + 1] - give[i]);
+      a.ring[ring_place(tail0, static_cast<int32_t>(j), a.num_pages)] =
           a.table[i * a.table_stride + keep + (j - give[i])];
     }
   }
-  // cursors_out may be cursors_in: the last block to have read them writes them
+  // where cursors_out is cursors_in, the last block to have read them writes them
   if (tid == 0) {
-    bool write = gridDim.x == 1;
-    if (!write) write = atomicAdd(a.arrived, 1) == static_cast<int>(gridDim.x) - 1;
+    bool write = blockIdx.x == 0;
+    if (a.arrived != nullptr) {
+      write = atomicAdd(a.arrived, 1) == static_cast<int>(gridDim.x) - 1;
+      if (write) st_dev(a.arrived, 0);
+    }
     if (write) {
-      if (gridDim.x > 1) st_dev(a.arrived, 0);
       a.cursors_out[0] = head + (status == 0 ? total[1] : 0);
       a.cursors_out[1] = tail + (status == 0 ? total[2] : 0);
       *a.status = status;
@@ -167,43 +189,82 @@ struct AppendArgs {
   void* q_out;
   f16 *keys, *values;
   int64_t page_stride;
-  int num_pages, page_shift, nkv, nq, hd;
+  int num_pages, page_shift, nkv, nq, hd, parts;
   const int32_t *positions, *slots;
 };
 
+// One row a block, or `parts` blocks where there are few rows: the units (rope.h) of the query heads, of the key heads,
+// then the value heads' W values each. The first unit is requested before slot and angles are known; a row without a
+// slot ends there. Bound by memory: 2531 rows of 16 query and 8 KV heads fp32 (72.6 MB) 13.1 us, 5.5 TB/s; 48 rows
+// of 32 and 8 by the launch: 5.5 us a call, 3.4 of them the kernel's (4.5 with one block a row).
 template <typename T, int W>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
   __shared__ f32x2 cs[64];  // head_dim <= 128
-  const int64_t r = blockIdx.x;
-  const int slot = checked_slot(a.slots[r], a.num_pages, a.page_shift);
-  if (slot < 0) return;
-  if (a.rope.turns != nullptr) rope_angles(a.rope, a.positions[r], cs);
-  __syncthreads();
-  const int units = rope_units(a.rope, W);
-  const int place = slot & ((1 << a.page_shift) - 1);
-  const int64_t page = static_cast<int64_t>(slot >> a.page_shift) * a.page_stride;
+  const int64_t r = blockIdx.x / a.parts;
+  const int units = rope_units(a.rope, W), copies = a.hd / W;
+  const int rotated = (a.nq + a.nkv) * units, all = rotated + a.nkv * copies;
   const T* q = static_cast<const T*>(a.q) + r * a.q_stride;
   const T* k = static_cast<const T*>(a.k) + r * a.k_stride;
   const T* v = static_cast<const T*>(a.v) + r * a.v_stride;
   T* q_out = static_cast<T*>(a.q_out) + r * a.q_out_stride;
-  const int rotated = (a.nq + a.nkv) * units, copied = a.nkv * (a.hd / W);
-  for (int u = threadIdx.x; u < rotated + copied; u += blockDim.x) {
-    if (u < rotated) {
-      const int h = u / units, w = u - h * units;
-      if (h < a.nq) {
-        rope_unit<T, T, W>(a.rope, cs, q + h * a.hd, q_out + h * a.hd, w);
-      } else {
-        const int g = h - a.nq;
-        f16* dst = a.keys + page + ((static_cast<int64_t>(g) << a.page_shift) + place) * a.hd;
-        rope_unit<T, f16, W>(a.rope, cs, k + g * a.hd, dst, w);
-      }
+  const int first = (blockIdx.x % a.parts) * 256 + threadIdx.x, step = a.parts * 256;
+  auto load = [&](int u) {
+    RopeUnit<T, W> unit;
+    if (u >= rotated) {
+      unit.a = unit.b = load_vec<T, W>(v + (u - rotated) * W);
     } else {
-      const int w = u - rotated, g = w / (a.hd / W), d = (w - g * (a.hd / W)) * W;
-      float x[W];
-      load_vec<T, W>(v + g * a.hd + d, x);
-      store_vec<f16, W>(a.values + page + ((static_cast<int64_t>(g) << a.page_shift) + place) * a.hd + d, x);
+      const int h = u / units;
+      unit = load_unit<T, W>(a.rope, h < a.nq ? q + h * a.hd : k + (h - a.nq) * a.hd, u - h * units);
+    }
+    return unit;
+  };
+  RopeUnit<T, W> unit = load(min(first, all - 1));
+  const int slot = checked_slot(a.slots[r], a.num_pages, a.page_shift);
+  if (slot < 0) return;
+  if (a.rope.turns != nullptr) rope_angles(a.rope, a.positions[r], cs);
+  __syncthreads();
+  const int place = slot & ((1 << a.page_shift) - 1);
+  const int64_t page = static_cast<int64_t>(slot >> a.page_shift) * a.page_stride;
+  auto cached = [&](f16* pool, int g) { return pool + page + ((static_cast<int64_t>(g) << a.page_shift) + place) * a.hd; };
+  for (int u = first; u < all; u += step) {
+    if (u != first) unit = load(u);
+    const int h = u / units, w = u - h * units;
+    if (u >= rotated) {
+      const int c = u - rotated, g = c / copies;
+      store_copy<T, f16, W>(unit, cached(a.values, g) + (c - g * copies) * W);
+    } else if (h < a.nq) {
+      store_unit<T, T, W>(a.rope, cs, unit, q_out + h * a.hd, w);
+    } else {
+      store_unit<T, f16, W>(a.rope, cs, unit, cached(a.keys, h - a.nq), w);
     }
   }
+}
+
+template <typename T>
+hipError_t launch_paged_append(AppendArgs a, int64_t rows, hipStream_t s) {
+  constexpr int W = 16 / sizeof(T);
+  const bool aligned = aligned_rows(a.k, a.k_stride, sizeof(T)) && aligned_rows(a.v, a.v_stride, sizeof(T)) &&
+                       (a.nq == 0 || (aligned_rows(a.q, a.q_stride, sizeof(T)) &&
+                                      aligned_rows(a.q_out, a.q_out_stride, sizeof(T))));
+  const int w = aligned && wide_units(a.rope, W) ? W : aligned && wide_units(a.rope, 4) ? 4 : 1;
+  auto* kernel = w == W ? k_paged_append<T, W> : w == 4 ? k_paged_append<T, 4> : k_paged_append<T, 1>;
+  const int64_t units = (a.nq + a.nkv) * (a.rope.rotary_dim / (2 * w) + (a.hd - a.rope.rotary_dim) / w) +
+                        a.nkv * (a.hd / w);
+  a.parts = row_blocks(rows, units);
+  for (int64_t r = 0; r < rows; r += kRowsALaunch) {
+    AppendArgs b = a;
+    if (a.nq > 0) b.q = static_cast<const T*>(a.q) + r * a.q_stride;
+    b.k = static_cast<const T*>(a.k) + r * a.k_stride;
+    b.v = static_cast<const T*>(a.v) + r * a.v_stride;
+    if (a.nq > 0) b.q_out = static_cast<T*>(a.q_out) + r * a.q_out_stride;
+    if (a.rope.turns != nullptr) b.positions = a.positions + r;
+    b.slots = a.slots + r;
+    const int n = static_cast<int>(std::min<int64_t>(kRowsALaunch, rows - r));
+    hipLaunchKernelGGL(kernel, dim3(n * a.parts), dim3(256), 0, s, b);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 // ---- decode attention ------------------------------------------------------------------------------------------------
@@ -261,7 +322,7 @@ __device__ __forceinline__ float across_rows(float x, F f) {
 __device__ __forceinline__ float both_parts(float x) { return x + dpp_mov<0x128>(x); }
 
 template <typename T, int HD, int NT>
-__global__ __launch_bounds__(256, HD == 64 ? 4 : NT == 1 ? 3 : 2) void k_paged_attention(PagedAttnArgs a) {
+__global__ __launch_bounds__(256, NT == 2 && HD == 128 ? 2 : HD == 64 && NT == 1 ? 4 : 3) void k_paged_attention(PagedAttnArgs a) {
   constexpr int KC = HD / 32;  // 32-dim steps of a score
   constexpr int VD = HD / 16;  // dims of a value row a lane reads: 8 (16 bytes) or 4
   constexpr int HEADS = 8 * NT;
@@ -614,10 +675,10 @@ int64_t page_stride(const soc_paged_cache* c) {
   return c->page_stride != 0 ? c->page_stride : static_cast<int64_t>(c->kv_heads) * c->page_size * c->head_dim;
 }
 
-int check_cache_memory(const soc_ctx* ctx, const soc_paged_cache* c) {
+int check_cache_memory(Operands& operands, const soc_paged_cache* c) {
   const int64_t page = static_cast<int64_t>(c->kv_heads) * c->page_size * c->head_dim;
-  SOC_TRY(check_device_rows(ctx, "paged cache keys", c->keys, c->num_pages, page_stride(c), page, 2));
-  return check_device_rows(ctx, "paged cache values", c->values, c->num_pages, page_stride(c), page, 2);
+  SOC_TRY(operands.rows("paged cache keys", c->keys, c->num_pages, page_stride(c), page, 2));
+  return operands.rows("paged cache values", c->values, c->num_pages, page_stride(c), page, 2);
 }
 
 int hip_status(hipError_t e, const char* what) {
@@ -634,7 +695,6 @@ int soc_paged_plan(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const int32
                    const int64_t* cursors_in, int64_t* cursors_out, int32_t* row_starts, int32_t* positions,
                    int32_t* slots, int32_t max_rows, int32_t* status) {
   SOC_API_BEGIN
-  using soc::check_device_rows;
   if (n <= 0 || n > soc::kPlanMaxRequests) return soc::fail(SOC_ERR_INVALID, "paged plan: 1 to 4096 requests");
   SOC_TRY(soc::check_page_size(page_size));
   if (max_pages <= 0 || max_pages > soc::kPlanMaxPages)
@@ -645,22 +705,31 @@ int soc_paged_plan(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const int32
     return soc::fail(SOC_ERR_INVALID, "paged plan: need num_pages > 0 and num_pages * page_size below 2^31");
   if (ctx == nullptr) return soc::fail(SOC_ERR_INVALID, "null context");
   soc::DeviceScope device(ctx);
-  SOC_TRY(check_device_rows(ctx, "paged plan old_lens", old_lens, n, 1, 1, 4));
-  SOC_TRY(check_device_rows(ctx, "paged plan new_lens", new_lens, n, 1, 1, 4));
-  SOC_TRY(check_device_rows(ctx, "paged plan block_table", block_table, n, table_stride, max_pages, 4));
-  SOC_TRY(check_device_rows(ctx, "paged plan free_ring", free_ring, num_pages, 1, 1, 4));
-  SOC_TRY(check_device_rows(ctx, "paged plan cursors_in", cursors_in, 2, 1, 1, 8));
-  SOC_TRY(check_device_rows(ctx, "paged plan cursors_out", cursors_out, 2, 1, 1, 8));
-  SOC_TRY(check_device_rows(ctx, "paged plan row_starts", row_starts, n + 1, 1, 1, 4));
-  SOC_TRY(check_device_rows(ctx, "paged plan positions", positions, max_rows, 1, 1, 4));
-  SOC_TRY(check_device_rows(ctx, "paged plan slots", slots, max_rows, 1, 1, 4));
-  SOC_TRY(check_device_rows(ctx, "paged plan status", status, 1, 1, 1, 4));
-  SOC_TRY(soc::ensure_serve_ws(ctx, 0, 64));
-  soc::PlanArgs a{n,          old_lens,  new_lens,  block_table, max_pages, table_stride, free_ring,
-                  num_pages,  soc::shift_of(page_size), cursors_in, cursors_out, row_starts, positions, slots,
-                  max_rows,   status,    ctx->serve_counters};
+  soc::Operands operands(ctx);
+  SOC_TRY(operands.array("paged plan old_lens", old_lens, n, 4));
+  SOC_TRY(operands.array("paged plan new_lens", new_lens, n, 4));
+  SOC_TRY(operands.rows("paged plan block_table", block_table, n, table_stride, max_pages, 4));
+  SOC_TRY(operands.array("paged plan free_ring", free_ring, num_pages, 4));
+  SOC_TRY(operands.array("paged plan cursors_in", cursors_in, 2, 8));
+  SOC_TRY(operands.array("paged plan cursors_out", cursors_out, 2, 8));
+  SOC_TRY(operands.array("paged plan row_starts", row_starts, n + 1, 4));
+  SOC_TRY(operands.array("paged plan positions", positions, max_rows, 4));
+  SOC_TRY(operands.array("paged plan slots", slots, max_rows, 4));
+  SOC_TRY(operands.array("paged plan status", status, 1, 4));
+  // a row a thread
   const int blocks = std::min(256, std::max(1, (max_rows + soc::kPlanThreads - 1) / soc::kPlanThreads));
-  hipLaunchKernelGGL(soc::k_paged_plan, dim3(blocks), dim3(soc::kPlanThreads), 0, ctx->stream, a);
+  int* arrived = nullptr;
+  if (blocks > 1 && cursors_out < cursors_in + 2 && cursors_in < cursors_out + 2) {
+    SOC_TRY(soc::ensure_serve_ws(ctx, 0, 1));
+    arrived = ctx->serve_counters;
+  }
+  soc::PlanArgs a{n,         old_lens, new_lens,   block_table, max_pages,
+                  table_stride, free_ring, num_pages, soc::shift_of(page_size), cursors_in,
+                  cursors_out, row_starts, positions, slots, max_rows, status, arrived};
+  auto* kernel = n <= soc::kPlanThreads       ? soc::k_paged_plan<1>
+                 : n <= 4 * soc::kPlanThreads ? soc::k_paged_plan<4>
+                                              : soc::k_paged_plan<soc::kPlanMaxRequests / soc::kPlanThreads>;
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(soc::kPlanThreads), 0, ctx->stream, a);
   return soc::hip_status(hipGetLastError(), "paged plan");
   SOC_API_END
 }
@@ -670,7 +739,6 @@ int soc_paged_append(soc_ctx* ctx, const soc_paged_cache* cache, const soc_rope*
                      int64_t q_out_stride, int32_t rows, int32_t q_heads, const int32_t* positions,
                      const int32_t* slots) {
   SOC_API_BEGIN
-  using soc::check_device_rows;
   SOC_TRY(soc::check_cache_shape(cache));
   if (dtype != SOC_DTYPE_F32 && dtype != SOC_DTYPE_F16)
     return soc::fail(SOC_ERR_INVALID, "paged append: dtype must be F32 or F16");
@@ -683,17 +751,18 @@ int soc_paged_append(soc_ctx* ctx, const soc_paged_cache* cache, const soc_rope*
   if (rope != nullptr && (rope->ctx != ctx || rope->head_dim != cache->head_dim))
     return soc::fail(SOC_ERR_INVALID, "paged append: the rope is of another context or head_dim");
   soc::DeviceScope device(ctx);
+  soc::Operands operands(ctx);
   const int size = dtype == SOC_DTYPE_F32 ? 4 : 2, hd = cache->head_dim;
   const int64_t kv = static_cast<int64_t>(cache->kv_heads) * hd, qw = static_cast<int64_t>(q_heads) * hd;
-  SOC_TRY(soc::check_cache_memory(ctx, cache));
-  SOC_TRY(check_device_rows(ctx, "paged append keys", k, rows, k_stride, kv, size));
-  SOC_TRY(check_device_rows(ctx, "paged append values", v, rows, v_stride, kv, size));
+  SOC_TRY(soc::check_cache_memory(operands, cache));
+  SOC_TRY(operands.rows("paged append keys", k, rows, k_stride, kv, size));
+  SOC_TRY(operands.rows("paged append values", v, rows, v_stride, kv, size));
   if (q_heads > 0) {
-    SOC_TRY(check_device_rows(ctx, "paged append queries", q, rows, q_stride, qw, size));
-    if (q_out != q) SOC_TRY(check_device_rows(ctx, "paged append q_out", q_out, rows, q_out_stride, qw, size));
+    SOC_TRY(operands.rows("paged append queries", q, rows, q_stride, qw, size));
+    if (q_out != q) SOC_TRY(operands.rows("paged append q_out", q_out, rows, q_out_stride, qw, size));
   }
-  if (rope != nullptr) SOC_TRY(check_device_rows(ctx, "paged append positions", positions, rows, 1, 1, 4));
-  SOC_TRY(check_device_rows(ctx, "paged append slots", slots, rows, 1, 1, 4));
+  if (rope != nullptr) SOC_TRY(operands.array("paged append positions", positions, rows, 4));
+  SOC_TRY(operands.array("paged append slots", slots, rows, 4));
   soc::AppendArgs a{};
   a.rope = soc::view_of(rope, hd);
   a.q = q;
@@ -714,13 +783,9 @@ int soc_paged_append(soc_ctx* ctx, const soc_paged_cache* cache, const soc_rope*
   a.hd = hd;
   a.positions = positions;
   a.slots = slots;
-  const bool wide = soc::four_wide(a.rope) && soc::four_wide(k, k_stride, size) && soc::four_wide(v, v_stride, size) &&
-                    (q_heads == 0 ||
-                     (soc::four_wide(q, q_stride, size) && soc::four_wide(q_out, q_out_stride, size)));
-  auto* kernel = size == 4 ? (wide ? soc::k_paged_append<float, 4> : soc::k_paged_append<float, 1>)
-                           : (wide ? soc::k_paged_append<soc::f16, 4> : soc::k_paged_append<soc::f16, 1>);
-  hipLaunchKernelGGL(kernel, dim3(rows), dim3(256), 0, ctx->stream, a);
-  return soc::hip_status(hipGetLastError(), "paged append");
+  const hipError_t e = size == 4 ? soc::launch_paged_append<float>(a, rows, ctx->stream)
+                                 : soc::launch_paged_append<soc::f16>(a, rows, ctx->stream);
+  return soc::hip_status(e, "paged append");
   SOC_API_END
 }
 
@@ -729,7 +794,6 @@ int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const
                                const int32_t* seq_lens, int32_t n, int32_t q_heads, float scale, void* out,
                                int64_t out_stride, float* lse) {
   SOC_API_BEGIN
-  using soc::check_device_rows;
   SOC_TRY(soc::check_cache_shape(cache));
   if (dtype != SOC_DTYPE_F32 && dtype != SOC_DTYPE_F16)
     return soc::fail(SOC_ERR_INVALID, "paged attention: dtype must be F32 or F16");
@@ -743,14 +807,15 @@ int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const
     return soc::fail(SOC_ERR_INVALID, "paged attention: in place needs equal strides");
   if (ctx == nullptr) return soc::fail(SOC_ERR_INVALID, "null context");
   soc::DeviceScope device(ctx);
+  soc::Operands operands(ctx);
   const int size = dtype == SOC_DTYPE_F32 ? 4 : 2, hd = cache->head_dim;
   const int64_t width = static_cast<int64_t>(q_heads) * hd;
-  SOC_TRY(soc::check_cache_memory(ctx, cache));
-  SOC_TRY(check_device_rows(ctx, "paged attention queries", q, n, q_stride, width, size));
-  if (out != q) SOC_TRY(check_device_rows(ctx, "paged attention output", out, n, out_stride, width, size));
-  SOC_TRY(check_device_rows(ctx, "paged attention block_table", block_table, n, table_stride, max_pages, 4));
-  SOC_TRY(check_device_rows(ctx, "paged attention seq_lens", seq_lens, n, 1, 1, 4));
-  if (lse != nullptr) SOC_TRY(check_device_rows(ctx, "paged attention lse", lse, n, q_heads, q_heads, 4));
+  SOC_TRY(soc::check_cache_memory(operands, cache));
+  SOC_TRY(operands.rows("paged attention queries", q, n, q_stride, width, size));
+  if (out != q) SOC_TRY(operands.rows("paged attention output", out, n, out_stride, width, size));
+  SOC_TRY(operands.rows("paged attention block_table", block_table, n, table_stride, max_pages, 4));
+  SOC_TRY(operands.array("paged attention seq_lens", seq_lens, n, 4));
+  if (lse != nullptr) SOC_TRY(operands.rows("paged attention lse", lse, n, q_heads, q_heads, 4));
   soc::PagedAttnArgs a{};
   a.keys = static_cast<const soc::f16*>(cache->keys);
   a.values = static_cast<const soc::f16*>(cache->values);
@@ -772,7 +837,7 @@ int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const
   a.wide_q = reinterpret_cast<uintptr_t>(q) % (8 * size) == 0 && q_stride % 8 == 0;
   a.n = n;
   const int64_t pairs = static_cast<int64_t>(n) * cache->kv_heads;
-  if (pairs > INT32_MAX / 256) return soc::fail(SOC_ERR_INVALID, "paged attention: too many sequences times KV heads");
+  if (pairs > (1 << 20)) return soc::fail(SOC_ERR_INVALID, "paged attention: sequences times KV heads beyond 2^20");
   const int64_t longest = static_cast<int64_t>(max_pages) * cache->page_size;
   const size_t part = static_cast<size_t>(a.group) * (hd + 2) * sizeof(float);
   const int64_t room = std::max<int64_t>(1, (int64_t{512} << 20) / static_cast<int64_t>(pairs * part));

@@ -47,10 +47,14 @@ SOC_HD int32_t attention_chunk(int32_t len, int32_t splits, int32_t most, int32_
   return chunk == 128 && len > 16 * 128 ? 256 : chunk;
 }
 
-// Place of entry number `cursor` + i of a ring of `size` entries, for any cursor.
-SOC_HD int32_t ring_place(int64_t cursor, int32_t i, int32_t size) {
-  const uint64_t at = static_cast<uint64_t>(cursor) % static_cast<uint64_t>(size) + static_cast<uint32_t>(i);
-  return static_cast<int32_t>(at % static_cast<uint64_t>(size));
+// Place of a cursor in a ring of `size` entries, for any cursor.
+SOC_HD int32_t ring_place(int64_t cursor, int32_t size) {
+  return static_cast<int32_t>(static_cast<uint64_t>(cursor) % static_cast<uint64_t>(size));
+}
+// Place of the entry i <= size (< 2^30) places on from `place`.
+SOC_HD int32_t ring_place(int32_t place, int32_t i, int32_t size) {
+  const int32_t at = place + i;
+  return at < size ? at : at - size < size ? at - size : 0;
 }
 
 // What a step asks for that brings a request from `before` to `after` positions: new rows, pages to take and to give

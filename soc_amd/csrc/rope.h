@@ -2,6 +2,8 @@
 // soc_rope_apply and soc_paged_append share.
 #pragma once
 
+#include <algorithm>
+
 #include "device_common.h"
 #include "soc_hip.h"
 
@@ -47,16 +49,14 @@ struct VecOf<T, 1> {
 };
 
 template <typename T, int W>
-__device__ __forceinline__ void load_vec(const T* p, float* x) {
-  const auto v = *reinterpret_cast<const typename VecOf<T, W>::type*>(p);
-  if constexpr (W == 1) {
-    x[0] = static_cast<float>(v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < W; ++i) x[i] = static_cast<float>(v[i]);
-  }
+__device__ __forceinline__ typename VecOf<T, W>::type load_vec(const T* p) {
+  return *reinterpret_cast<const typename VecOf<T, W>::type*>(p);
 }
-
+template <typename T, int W>
+__device__ __forceinline__ float element(typename VecOf<T, W>::type v, int i) {
+  if constexpr (W == 1) return static_cast<float>(v);
+  else return static_cast<float>(v[i]);
+}
 template <typename T, int W>
 __device__ __forceinline__ void store_vec(T* p, const float* x) {
   typename VecOf<T, W>::type v;
@@ -69,42 +69,58 @@ __device__ __forceinline__ void store_vec(T* p, const float* x) {
   *reinterpret_cast<typename VecOf<T, W>::type*>(p) = v;
 }
 
-// Units a head is worked in: W pairs together (2 W values), then the values behind the rotated ones, W a unit.
+// Units a head is worked in: W pairs together (2 W values), then the values behind the rotated ones, W a unit. A unit's
+// values are all read before any of them is written, and no other unit touches them: in place is fine.
 __device__ __forceinline__ int rope_units(const RopeView& v, int w) {
   return v.rotary_dim / (2 * w) + (v.head_dim - v.rotary_dim) / w;
 }
+template <typename T, int W>
+struct RopeUnit {
+  typename VecOf<T, W>::type a, b;  // the pairs' first and second values (interleaved: as they lie); or a to copy
+};
 
-// Unit u of one head: x -> y (another type where y is the cache's). y may be x: a unit's values are read before any of
-// them is written, and no other unit touches them.
+template <typename T, int W>
+__device__ __forceinline__ RopeUnit<T, W> load_unit(const RopeView& v, const T* x, int u) {
+  const int pair_units = v.rotary_dim / (2 * W);
+  const bool pairs = u < pair_units;
+  const int at = !pairs ? v.rotary_dim + (u - pair_units) * W : v.interleaved ? 2 * W * u : W * u;
+  RopeUnit<T, W> r;
+  r.a = load_vec<T, W>(x + at);
+  r.b = load_vec<T, W>(x + at + (!pairs ? 0 : v.interleaved ? W : v.rotary_dim / 2));
+  return r;
+}
+
+// W values of a unit as they are.
 template <typename T, typename O, int W>
-__device__ __forceinline__ void rope_unit(const RopeView& v, const f32x2* cs, const T* x, O* y, int u) {
+__device__ __forceinline__ void store_copy(const RopeUnit<T, W>& r, O* y) {
+  float x[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) x[i] = element<T, W>(r.a, i);
+  store_vec<O, W>(y, x);
+}
+
+// Unit u, rotated, to y (O: another type where y is the cache's). Written as explicit fmaf, so that every width computes
+// the same bits.
+template <typename T, typename O, int W>
+__device__ __forceinline__ void store_unit(const RopeView& v, const f32x2* cs, const RopeUnit<T, W>& r, O* y, int u) {
   const int pair_units = v.rotary_dim / (2 * W);
   if (u >= pair_units) {
-    const int at = v.rotary_dim + (u - pair_units) * W;
-    float a[W];
-    load_vec<T, W>(x + at, a);
-    store_vec<O, W>(y + at, a);
+    store_copy<T, O, W>(r, y + v.rotary_dim + (u - pair_units) * W);
     return;
   }
-  float a[W], b[W], p[W], q[W];
-  if (v.interleaved) {
-    float m[2 * W];
-    load_vec<T, W>(x + 2 * W * u, m);
-    load_vec<T, W>(x + 2 * W * u + W, m + W);
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      a[i] = m[2 * i];
-      b[i] = m[2 * i + 1];
-    }
-  } else {
-    load_vec<T, W>(x + W * u, a);
-    load_vec<T, W>(x + v.rotary_dim / 2 + W * u, b);
-  }
+  float p[W], q[W];
 #pragma unroll
   for (int i = 0; i < W; ++i) {
     const f32x2 t = cs[W * u + i];
-    p[i] = a[i] * t[0] - b[i] * t[1];
-    q[i] = b[i] * t[0] + a[i] * t[1];
+    float a = element<T, W>(r.a, i), b = element<T, W>(r.b, i);
+    if (v.interleaved) {  // pair i of the 2 W values a, b
+      if constexpr (W > 1) {
+        a = 2 * i < W ? element<T, W>(r.a, (2 * i) % W) : element<T, W>(r.b, (2 * i) % W);
+        b = 2 * i + 1 < W ? element<T, W>(r.a, (2 * i + 1) % W) : element<T, W>(r.b, (2 * i + 1) % W);
+      }
+    }
+    p[i] = fmaf(a, t[0], -(b * t[1]));
+    q[i] = fmaf(a, t[1], b * t[0]);
   }
   if (v.interleaved) {
     float m[2 * W];
@@ -126,11 +142,17 @@ inline RopeView view_of(const soc_rope* r, int head_dim) {
   return RopeView{r->turns, r->head_dim, r->rotary_dim, r->interleaved, r->gain};
 }
 
-// Whether rows of heads that start at p, `stride` elements apart, can be read and written four elements at a time.
-inline bool four_wide(const void* p, int64_t stride, int size) {
-  return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && stride % 4 == 0;
+// Values that one load or store takes: 16 bytes where rows that start at p, `stride` elements apart, allow it.
+inline bool aligned_rows(const void* p, int64_t stride, int size) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
 }
-// Whether a head's units can be four wide: pairs and the values behind them come in fours.
-inline bool four_wide(const RopeView& v) { return v.rotary_dim % 8 == 0 && v.head_dim % 4 == 0; }
+// Whether a head's units can be w wide: pairs, and the values behind them, come in w.
+inline bool wide_units(const RopeView& v, int w) { return v.rotary_dim % (2 * w) == 0 && v.head_dim % w == 0; }
+
+// Blocks a row of `units` is given: one for 256 of them while the card has CUs to spare, else one for all.
+inline int row_blocks(int64_t rows, int64_t units) {
+  return static_cast<int>(rows < 512 ? std::min<int64_t>((units + 255) / 256, (1024 + rows - 1) / rows) : 1);
+}
+constexpr int64_t kRowsALaunch = 1 << 20;  // rows of one launch: its work-items stay below 2^32
 
 }  // namespace soc

@@ -6,8 +6,7 @@
 
 namespace soc {
 
-int check_device_rows(const soc_ctx* ctx, const char* what, const void* p, int64_t rows, int64_t stride, int64_t width,
-                      int size) {
+int Operands::rows(const char* what, const void* p, int64_t rows, int64_t stride, int64_t width, int size) {
   if (rows <= 0 || width <= 0) return SOC_OK;
   if (p == nullptr) return fail(SOC_ERR_INVALID, std::string(what) + ": null device pointer");
   if (stride < width || stride > (int64_t{1} << 40))
@@ -17,25 +16,33 @@ int check_device_rows(const soc_ctx* ctx, const char* what, const void* p, int64
   // rows < 2^31 and stride <= 2^40 could pass 64 bits of bytes: no allocation is that large
   const unsigned __int128 bytes =
       (static_cast<unsigned __int128>(rows - 1) * static_cast<uint64_t>(stride) + static_cast<uint64_t>(width)) * size;
-  if (bytes > (static_cast<unsigned __int128>(1) << 46))
-    return fail(SOC_ERR_INVALID, std::string(what) + " extends past the end of its device allocation");
-  hipPointerAttribute_t attr{};
-  if (hipPointerGetAttributes(&attr, p) != hipSuccess) {
-    (void)hipGetLastError();
-    return fail(SOC_ERR_INVALID, std::string(what) + " is not in device memory");
+  const char* begin = static_cast<const char*>(p);
+  const Range* in = nullptr;
+  for (int i = 0; i < count_ && in == nullptr; ++i)
+    if (begin >= known_[i].begin && begin < known_[i].end) in = &known_[i];
+  Range asked{nullptr, nullptr};
+  if (in == nullptr) {
+    hipPointerAttribute_t attr{};
+    if (hipPointerGetAttributes(&attr, p) != hipSuccess) {
+      (void)hipGetLastError();
+      return fail(SOC_ERR_INVALID, std::string(what) + " is not in device memory");
+    }
+    if ((attr.type == hipMemoryTypeHost && attr.devicePointer != p) ||
+        (attr.type != hipMemoryTypeDevice && attr.type != hipMemoryTypeManaged && attr.type != hipMemoryTypeHost))
+      return fail(SOC_ERR_INVALID, std::string(what) + " is not in device memory");
+    if (attr.type == hipMemoryTypeDevice && attr.device != ctx_->device)
+      return fail(SOC_ERR_INVALID, std::string(what) + " is memory of another device than the context's");
+    void* base = nullptr;
+    size_t held = 0;
+    if (hipMemGetAddressRange(&base, &held, const_cast<void*>(p)) != hipSuccess) {
+      (void)hipGetLastError();
+      return fail(SOC_ERR_INVALID, std::string(what) + " extends past the end of its device allocation");
+    }
+    asked = Range{static_cast<const char*>(base), static_cast<const char*>(base) + held};
+    in = &asked;
+    if (count_ < static_cast<int>(sizeof(known_) / sizeof(known_[0]))) known_[count_++] = asked;
   }
-  if ((attr.type == hipMemoryTypeHost && attr.devicePointer != p) ||
-      (attr.type != hipMemoryTypeDevice && attr.type != hipMemoryTypeManaged && attr.type != hipMemoryTypeHost))
-    return fail(SOC_ERR_INVALID, std::string(what) + " is not in device memory");
-  if (attr.type == hipMemoryTypeDevice && attr.device != ctx->device)
-    return fail(SOC_ERR_INVALID, std::string(what) + " is memory of another device than the context's");
-  void* base = nullptr;
-  size_t held = 0;
-  if (hipMemGetAddressRange(&base, &held, const_cast<void*>(p)) != hipSuccess) {
-    (void)hipGetLastError();
-    return fail(SOC_ERR_INVALID, std::string(what) + " extends past the end of its device allocation");
-  }
-  if (static_cast<const char*>(p) + static_cast<size_t>(bytes) > static_cast<const char*>(base) + held)
+  if (bytes > static_cast<uint64_t>(in->end - begin))
     return fail(SOC_ERR_INVALID, std::string(what) + " extends past the end of its device allocation");
   return SOC_OK;
 }

@@ -72,10 +72,10 @@ int main() {
   }
   for (int i = 0; i < 200000; ++i) {
     const int64_t cursor = static_cast<int64_t>(rng() >> (rng() % 64)) * (i % 2 ? 1 : -1);
-    const int32_t size = 1 + static_cast<int32_t>((rng() >> 33) >> (rng() % 31)) % (INT32_MAX - 1);
-    const int32_t at = static_cast<int32_t>(rng() >> 33) % size;
-    const int32_t place = soc::ring_place(cursor, at, size);
-    expect(place >= 0 && place < size, "ring_place is in the ring");
+    const int32_t size = 1 + static_cast<int32_t>((rng() >> 33) >> (rng() % 31)) % ((1 << 27) - 1);
+    const int32_t at = static_cast<int32_t>(rng() >> 33) % (size + 1);
+    const int32_t base = soc::ring_place(cursor, size), place = soc::ring_place(base, at, size);
+    expect(base >= 0 && base < size && place >= 0 && place < size, "ring_place is in the ring");
     if (cursor >= 0 && cursor < (int64_t{1} << 62))
       expect(place == static_cast<int32_t>((cursor + at) % size), "ring_place is the sum modulo the size");
   }
