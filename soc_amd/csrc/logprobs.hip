@@ -433,7 +433,7 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
     return soc::fail(SOC_ERR_INVALID, "logprobs: need rows > 0 and a vocabulary of 1 to 2^20");
   if (top_n < 0 || top_n > soc::kMaxTop || top_n > vocab)
     return soc::fail(SOC_ERR_INVALID, "logprobs: top_n must be 0 to min(64, vocab)");
-  if (!std::isfinite(temperature) || (temperature > 0.0f && !std::isfinite(1.0f / temperature)))
+  if (!std::isfinite(temperature) || (temperature > 0.0f && !std::isfinite(2.0f / temperature)))
     return soc::fail(SOC_ERR_INVALID, "logprobs: temperature and its inverse must be finite");
   if (tokens == nullptr && (logprobs != nullptr || ranks != nullptr))
     return soc::fail(SOC_ERR_INVALID, "logprobs: log probabilities and ranks need tokens");
@@ -462,8 +462,8 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
   const int each = (chunks_of(64) == 1 && chunks_of(32) > 1) || vocab > (1 << 18) ? 64 : 32;
   const int chunks = chunks_of(each);
   const size_t per_row = chunks > 1 ? chunks * (sizeof(soc::Part) + static_cast<size_t>(top_n) * 8) : 0;
-  // rows a launch: its workspace stays below 256 MiB, its work-items below 2^32
-  const int64_t most = std::min<int64_t>(std::max<int64_t>(1, (int64_t{256} << 20) / std::max<size_t>(1, per_row)),
+  // rows a launch: its workspace stays below 32 MiB, its work-items below 2^32
+  const int64_t most = std::min<int64_t>(std::max<int64_t>(1, (int64_t{32} << 20) / std::max<size_t>(1, per_row)),
                                          (int64_t{1} << 23) / chunks);
   const int step = static_cast<int>(std::min<int64_t>(rows, most));
   if (chunks > 1) SOC_TRY(soc::ensure_serve_ws(ctx, step * per_row, step));

@@ -125,7 +125,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PlanArgs a) {
     give[a.n] = total[2];
   }
   __syncthreads();
-  const int64_t free_pages = tail - head;
+  // any words may stand there: the difference wraps, and is looked at only where both are counts
+  const int64_t free_pages = static_cast<int64_t>(static_cast<uint64_t>(tail) - static_cast<uint64_t>(head));
   int status = any_bad ? SOC_PLAN_LENGTHS : 0;
   if (head < 0 || tail < 0 || free_pages < 0 || free_pages > a.num_pages) status |= SOC_PLAN_CURSORS;
   else if (free_pages + total[2] > a.num_pages) status |= SOC_PLAN_CURSORS;
@@ -174,8 +175,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PlanArgs a) {
       if (write) st_dev(a.arrived, 0);
     }
     if (write) {
-      a.cursors_out[0] = head + (status == 0 ? total[1] : 0);
-      a.cursors_out[1] = tail + (status == 0 ? total[2] : 0);
+      a.cursors_out[0] = status == 0 ? head + total[1] : head;
+      a.cursors_out[1] = status == 0 ? tail + total[2] : tail;
       *a.status = status;
     }
   }
