@@ -2536,8 +2536,6 @@ int ensure_op_attention_ws(soc_ctx* ctx, size_t floats, size_t ints) {
   if (ctx->op_counter_ints < ints) {
     if ((e = hipStreamSynchronize(ctx->stream)) != hipSuccess) return hip_fail(e, "hipStreamSynchronize");
     (void)hipFree(ctx->op_counters);
-  (void)hipFree(ctx->serve_ws);
-  (void)hipFree(ctx->serve_counters);
     ctx->op_counters = nullptr;
     ctx->op_counter_ints = 0;
     if ((e = hipMalloc(&ctx->op_counters, ints * 4)) != hipSuccess) return hip_fail(e, "hipMalloc attention counters");

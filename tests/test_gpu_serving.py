@@ -191,3 +191,26 @@ def test_logprobs_of_more_rows_than_a_launch(gpu_ctx):
         assert torch.equal(ids[at].long(), best.indices[:, :top])
         place = (best.indices == t[at].long()[:, None]).int().argmax(-1)
         assert torch.equal(rk[at].long(), place)
+
+
+def test_workspaces_of_other_operators_growing_in_between(gpu_ctx):
+    """The contiguous attention's scratch, grown between the paged calls, leaves theirs alone."""
+    ctx = S.Context(0)
+    try:
+        with Arrays(ctx) as mem:
+            jobs = [Attention(ctx, mem, 21, 3, 3000), Logprobs(ctx, mem, 22, 3, 40000)]
+            for nkv, cap in ((2, 600), (8, 5000), (32, 5000)):
+                for j in jobs:
+                    j.queue()
+                plane = mem.up(np.ones((nkv, cap, 128), np.float16))
+                q, out = mem.up(np.ones((nkv, 128), np.float32)), mem.up(np.zeros((nkv, 128), np.float32))
+                S.attention_decode(ctx, q, plane, plane, out, cap, nkv, nkv, cap)
+                held = [mem.up(np.full(1024, 55, np.int32)) for _ in range(8)]  # takes what was freed, if anything was
+                for j in jobs:
+                    j.queue()
+                    assert j.wrong() < OFF
+                for p in held:
+                    assert (mem.down(p) == 55).all()
+                assert np.array_equal(mem.down(out), np.ones((nkv, 128), np.float32))
+    finally:
+        ctx.close()
