@@ -348,23 +348,27 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
     __syncthreads();
     if (!last) return;
     if (tid == 0) st_dev(a.arrived + r, 0);
+    // every wave the same sums, lane l parts l and l + 64 (at most 65): requested with the keys
+    Part mine[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int u = lane + j * kWave;
+      mine[j] = Part{-INFINITY, 0.0f, 0.0f, 0};
+      if (u < a.chunks) mine[j] = Part{ld_dev(&part[u].m), ld_dev(&part[u].s), ld_dev(&part[u].d), ld_dev(&part[u].above)};
+    }
     for (int i = tid; i < a.chunks * n; i += kThreads)
       keys[i] = __hip_atomic_load(tops + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // every wave the same sums
-    m = -INFINITY;
-    for (int u = lane; u < a.chunks; u += kWave) m = fmaxf(m, ld_dev(&part[u].m));
-    m = wave_max(m);
+    m = wave_max(fmaxf(mine[0].m, mine[1].m));
     s = d = 0.0f;
-    float counted = 0.0f;  // exact: at most 2^20
-    for (int u = lane; u < a.chunks; u += kWave) {
-      const float su = ld_dev(&part[u].s), du = ld_dev(&part[u].d), mu = ld_dev(&part[u].m);
-      const float shift = mu == -INFINITY ? -1000.0f : fmaxf((mu - m) * to_log2, -1000.0f);
-      const float f = __builtin_amdgcn_exp2f(shift);
-      s += su * f;
-      d += f * (du + shift * su);
-      if (su != su) s = su;
-      counted += static_cast<float>(ld_dev(&part[u].above));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const Part& p = mine[j];
+      const float shift = p.m == -INFINITY ? -1000.0f : fmaxf((p.m - m) * to_log2, -1000.0f);
+      const float f = __builtin_amdgcn_exp2f(shift);  // a NaN sum stays one: 0 times NaN is NaN
+      s += p.s * f;
+      d += f * (p.d + shift * p.s);
     }
+    const float counted = static_cast<float>(mine[0].above + mine[1].above);  // exact: at most 2^20
     s = wave_sum(s);
     d = wave_sum(d);
     above = static_cast<int>(wave_sum(counted));
