@@ -319,12 +319,17 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
     if (group[tid] >= t) {  // at most n threads
       const float tv = value_of<T>(static_cast<uint32_t>(t >> 32));
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (!(v[e] < tv)) {
-          const int id = place(e);
-          const uint64_t key = key_of<T>(v[e], id);
-          if (id >= 0 && id < a.vocab && key >= t) keys[atomicAdd(&found, 1)] = key;
-        }
+      for (int q = 0; q < E; q += 4) {  // four at a time: a thread has a candidate or two among its logits
+        const float most = fmaxf(fmaxf(v[q], v[q + 1]), fmaxf(v[q + 2], v[q + 3]));
+        if (most < tv && s == s) continue;
+#pragma unroll
+        for (int e = q; e < q + 4; ++e)
+          if (!(v[e] < tv)) {
+            const int id = place(e);
+            const uint64_t key = key_of<T>(v[e], id);
+            if (id >= 0 && id < a.vocab && key >= t) keys[atomicAdd(&found, 1)] = key;
+          }
+      }
     }
     __syncthreads();
     rank_first(keys, found, n, first);
