@@ -302,7 +302,7 @@ struct PagedAttnArgs {
   int64_t out_stride;
   float* lse;
   bool wide_q;             // query rows are 32-byte aligned (16 in fp16): eight values a load
-  int splits, most, grid;  // attention_chunk
+  int splits, grid;        // attention_chunk
   float* part;             // [n][nkv][grid][group * (HD + 2)]: outputs, then maxima, then sums
   int* arrived;            // [n][nkv], zero between launches
 };
@@ -328,7 +328,9 @@ __global__ __launch_bounds__(256, NT == 2 && HD == 128 ? 2 : HD == 64 && NT == 1
   constexpr int VD = HD / 16;  // dims of a value row a lane reads: 8 (16 bytes) or 4
   constexpr int HEADS = 8 * NT;
   typedef uint32_t VReg __attribute__((ext_vector_type(VD / 2)));
-  __shared__ float so[4][HEADS][HD], sm[4][HEADS], sl[4][HEADS];
+  // 4 floats behind a head's: 16-byte stores of 8 heads reach 8 bank groups
+  __shared__ alignas(16) float so[4][HEADS][HD + 4];
+  __shared__ float sm[4][HEADS], sl[4][HEADS];
   __shared__ float weight[256][HEADS], sums[256][HEADS];  // of up to 256 chunks
   __shared__ int last;
 
@@ -369,11 +371,10 @@ __global__ __launch_bounds__(256, NT == 2 && HD == 128 ? 2 : HD == 64 && NT == 1
     if (lse != nullptr && tid < G) lse[tid] = len < 0 ? nan : -INFINITY;
     return;
   }
-  const int chunk = attention_chunk(len, a.splits, a.most, a.grid);
-  const int blocks = (len - 1) / chunk + 1;
-  if (s >= blocks) return;
-  if (s != 0) load_queries();
+  const int chunk = attention_chunk(len, a.splits, a.grid);
   const uint32_t c0 = static_cast<uint32_t>(s) * chunk;
+  if (c0 >= static_cast<uint32_t>(len)) return;
+  if (s != 0) load_queries();
   const int tiles = (min(chunk, len - static_cast<int>(c0)) - 1) / 32 + 1;
   const int mine = (tiles - wid + 3) / 4;  // this wave's: wid, wid + 4, ..
   const int32_t* table = a.table + b * a.table_stride;
@@ -419,12 +420,7 @@ __global__ __launch_bounds__(256, NT == 2 && HD == 128 ? 2 : HD == 64 && NT == 1
       }
     }
   };
-  if (mine > 0) {
-    load_keys(0);
-    load_values(0);
-  }
-
-  // the query columns
+  // the query columns, while the pages are looked up
   f16x8 qb[NT][KC];
   float to_log2[NT];  // score of the scaled query -> base-2 exponent
 #pragma unroll
@@ -439,10 +435,11 @@ __global__ __launch_bounds__(256, NT == 2 && HD == 128 ? 2 : HD == 64 && NT == 1
         big = fmaxf(big, fabsf(static_cast<float>(qr[t][c][i])));
       }
     big = across_rows(big, [](float u, float v) { return fmaxf(u, v); });
-    // the largest becomes 2^13 .. 2^14
-    const int e = big > 0.0f && big < INFINITY ? min(13 - ilogbf(big), 126) : 0;
-    const float up = ldexpf(1.0f, e);
-    to_log2[t] = ldexpf(a.scale * kLog2e, -e);
+    // times 2^e, by which the largest becomes 2^13 .. 2^14 (subnormal ones less, by 2^126); not where it is 0 or no number
+    const int exponent = static_cast<int>(__float_as_uint(big) >> 23);
+    const int e = big > 0.0f && exponent < 255 ? min(140 - exponent, 126) : 0;
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    to_log2[t] = a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
     for (int c = 0; c < KC; ++c)
 #pragma unroll
@@ -451,6 +448,11 @@ __global__ __launch_bounds__(256, NT == 2 && HD == 128 ? 2 : HD == 64 && NT == 1
         const f16 high = static_cast<f16>(v);
         qb[t][c][i] = col < 8 ? high : static_cast<f16>(v - static_cast<float>(high));
       }
+  }
+
+  if (mine > 0) {
+    load_keys(0);
+    load_values(0);
   }
 
   float m[NT], l[NT];
@@ -525,51 +527,60 @@ __global__ __launch_bounds__(256, NT == 2 && HD == 128 ? 2 : HD == 64 && NT == 1
     if (more) load_values(i + 1);
   }
 
-  // the four waves
+  // the four waves: brought to their common maximum, then added. A wave without a tile has m = -inf and adds 0; a score
+  // of NaN leaves NaN in the sums
+  if (row == 0 && col < 8)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) sm[wid][t * 8 + col] = m[t];
+  lost = __syncthreads_or(lost);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const float sum = across_rows(l[t], [](float u, float v) { return u + v; });
-    if (row == 0 && col < 8) {
-      sm[wid][t * 8 + col] = m[t];
-      sl[wid][t * 8 + col] = sum;
-    }
+    const int h = t * 8 + (col & 7);
+    const float top = fmaxf(fmaxf(sm[0][h], sm[1][h]), fmaxf(sm[2][h], sm[3][h]));
+    const float f = __builtin_amdgcn_exp2f(m[t] - top);
+    const float sum = across_rows(l[t], [](float u, float v) { return u + v; }) * f;
+    if (row == 0 && col < 8) sl[wid][h] = sum;
+    // both columns of a head hold its sums: the high one stores rows 0 and 1 of the lane's four, the low one 2 and 3
 #pragma unroll
-    for (int d = 0; d < VD; ++d)
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float v = both_parts(o[t][d][r]);
-        if (col < 8) so[wid][t * 8 + col][(row * 4 + r) * VD + d] = v;
+      for (int d = 0; d < VD; d += 4) {
+        f32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float a0 = both_parts(o[t][d + i][r]), a1 = both_parts(o[t][d + i][r + 2]);
+          x[i] = (col < 8 ? a0 : a1) * f;
+        }
+        *reinterpret_cast<f32x4*>(&so[wid][h][(row * 4 + r + (col < 8 ? 0 : 2)) * VD + d]) = x;
       }
   }
-  lost = __syncthreads_or(lost);
+  __syncthreads();
+  const int blocks = (len - 1) / chunk + 1;
   const int64_t pair = static_cast<int64_t>(b) * a.nkv + g;
   const int stride = G * (HD + 2);
   float* part = a.part + (pair * a.grid + s) * stride;
-  // wave 0 has a tile, so the maximum is a number (or NaN scores make the sums NaN)
-  auto joined = [&](int h, float* w) {
-    const float top = fmaxf(fmaxf(sm[0][h], sm[1][h]), fmaxf(sm[2][h], sm[3][h]));
+  for (int i = tid; i < G * HD / 2; i += 256) {
+    const int h = 2 * i / HD, d = 2 * i % HD;
+    f32x2 x = *reinterpret_cast<const f32x2*>(&so[0][h][d]);
+    float sum = sl[0][h];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) w[u] = sl[u][h] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(sm[u][h] - top);
-    return top;
-  };
-  for (int i = tid; i < G * HD; i += 256) {
-    const int h = i / HD, d = i % HD;
-    float w[4];
-    joined(h, w);
-    float x = 0.0f, sum = 0.0f;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      x += w[u] * so[u][h][d];
-      sum += w[u] * sl[u][h];
+    for (int u = 1; u < 4; ++u) {
+      const f32x2 y = *reinterpret_cast<const f32x2*>(&so[u][h][d]);
+      x[0] += y[0];
+      x[1] += y[1];
+      sum += sl[u][h];
     }
-    if (blocks == 1) out[i] = static_cast<T>(lost ? nan : x / sum);
-    else st_dev(part + i, x);
+    if (blocks == 1) {
+      out[2 * i] = static_cast<T>(lost ? nan : x[0] / sum);
+      out[2 * i + 1] = static_cast<T>(lost ? nan : x[1] / sum);
+    } else {
+      __hip_atomic_store(reinterpret_cast<uint64_t*>(part) + i, __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+    }
   }
   if (tid < G) {
-    float w[4], sum = 0.0f;
-    const float top = joined(tid, w);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) sum += w[u] * sl[u][tid];
+    const float top = fmaxf(fmaxf(sm[0][tid], sm[1][tid]), fmaxf(sm[2][tid], sm[3][tid]));
+    float sum = (sl[0][tid] + sl[1][tid]) + (sl[2][tid] + sl[3][tid]);
     if (lost) sum = nan;
     if (blocks > 1) {
       st_dev(part + G * HD + tid, top);
@@ -844,12 +855,11 @@ int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const
   const int64_t room = std::max<int64_t>(1, (int64_t{512} << 20) / static_cast<int64_t>(pairs * part));
   // Blocks of a sequence. `splits`: one for each CU where there are few sequences (8 x 1000 keys, 16 query and 8 KV
   // heads: 12.5 us so, 15.4 with half of them; 8 x 4000, 32 and 8: 27 us, 31 with twice and 34 with four times as many),
-  // but 32 at most (one of 16000 keys, 14 and 2 heads: 19 us with 32 parts a head, 29 with 128). `most`: no block takes
-  // more than 1024 keys, so that ragged lengths even out. `grid`: what is launched for each row of the table, by its
+  // but 32 at most (one of 16000 keys, 14 and 2 heads: 19 us with 32 parts a head, 29 with 128). No block takes more
+  // than 1024 keys, so that ragged lengths even out. `grid`: what is launched for each row of the table, by its
   // width alone; a large batch has 8 (64 rows of 200 keys in a table 32768 wide: 12 us, 41 with 32, most of them empty).
   a.splits = static_cast<int>(std::min<int64_t>(32, (256 + pairs - 1) / pairs));
-  a.most = 1024;
-  a.grid = static_cast<int>(std::min({std::max<int64_t>(a.splits, (longest + a.most - 1) / a.most),
+  a.grid = static_cast<int>(std::min({std::max<int64_t>(a.splits, (longest + soc::kAttentionMost - 1) / soc::kAttentionMost),
                                       std::max<int64_t>(8, 4096 / pairs), (longest + 127) / 128, room, int64_t{256}}));
   if (a.grid > 1) {
     SOC_TRY(soc::ensure_serve_ws(ctx, static_cast<size_t>(pairs) * a.grid * part, static_cast<size_t>(pairs)));

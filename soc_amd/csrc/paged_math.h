@@ -35,15 +35,18 @@ SOC_HD int32_t checked_length(int32_t len, int32_t max_pages, int page_shift) {
   return len < 0 ? 0 : pages_of(len, page_shift) > max_pages ? -1 : len;
 }
 
-// Keys a block of the decode attention takes of a sequence of `len` > 0 keys (most >= 256): whole tiles of 128 (32 for each of its four
-// waves), so that the sequence gets at least `splits` blocks while it has tiles for them, and no block more than `most`
-// keys; but never more than `grid` blocks. More than 16 blocks take 256 keys at least: joining parts costs more than
-// shorter chunks save (one sequence of 4071 keys, 32 query and 8 KV heads: 12.8 us with 16 blocks, 14.1 with 32).
-SOC_HD int32_t attention_chunk(int32_t len, int32_t splits, int32_t most, int32_t grid) {
-  int32_t want = (len - 1) / most + 1;
+// Keys a block of the decode attention takes of a sequence of `len` > 0 keys: whole tiles of 128 (32 for each of its four
+// waves), so that the sequence gets at least `splits` blocks while it has tiles for them, and no block more than
+// kAttentionMost keys; but never more than `grid` blocks. More than 16 blocks take 256 keys at least: joining parts costs
+// more than shorter chunks save (one sequence of 4071 keys, 32 query and 8 KV heads: 12.8 us with 16 blocks, 14.1 with
+// 32).
+constexpr int32_t kAttentionMost = 1024;
+SOC_HD int32_t attention_chunk(int32_t len, int32_t splits, int32_t grid) {
+  int32_t want = (len - 1) / kAttentionMost + 1;
   want = want > splits ? want : splits;
   want = want < grid ? want : grid;
-  const int32_t chunk = ((len - 1) / want / 128 + 1) * 128;
+  const int32_t each = want == 1 ? len - 1 : (len - 1) / want;
+  const int32_t chunk = (each / 128 + 1) * 128;
   return chunk == 128 && len > 16 * 128 ? 256 : chunk;
 }
 

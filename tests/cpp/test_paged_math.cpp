@@ -62,12 +62,12 @@ int main() {
   std::mt19937_64 rng(5);
   for (int i = 0; i < 200000; ++i) {
     const int32_t len = 1 + static_cast<int32_t>((rng() >> 33) >> (rng() % 31)) % (INT32_MAX - 256);
-    const int32_t splits = 1 + rng() % 200, most = 128 * (2 + rng() % 64), grid = 1 + rng() % 300;
-    const int64_t chunk = soc::attention_chunk(len, splits, most, grid), blocks = (len - 1) / chunk + 1;
+    const int32_t splits = 1 + rng() % 200, grid = 1 + rng() % 300;
+    const int64_t chunk = soc::attention_chunk(len, splits, grid), blocks = (len - 1) / chunk + 1;
     expect(chunk > 0 && chunk % 128 == 0, "a chunk is whole tiles");
     expect(blocks <= grid, "the grid holds a sequence's blocks");
     expect((blocks - 1) * chunk < len, "no block is empty");
-    if ((int64_t{len} - 1) / most + 1 <= grid) expect(chunk <= most, "no block takes more than it may");
+    if ((int64_t{len} - 1) / soc::kAttentionMost + 1 <= grid) expect(chunk <= soc::kAttentionMost, "no block takes more than it may");
     if (len > 128 * splits && splits <= grid) expect(blocks * 2 >= splits, "a long sequence gets its blocks");
   }
   for (int i = 0; i < 200000; ++i) {
