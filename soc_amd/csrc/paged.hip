@@ -285,9 +285,8 @@ hipError_t launch_paged_append(AppendArgs a, int64_t rows, hipStream_t s) {
 //           the columns as the queries are, and scaled by 2^14 so that small weights stay normal fp16 numbers.
 // Keys behind the sequence's end are read as its last key and get weight 0: what memory holds there is never used.
 //
-// Bound by memory: 200 sequences up to 8192 keys (3.4 GB) 561 us, 6.06 TB/s (a large copy: 4.8); 48 up to 1500 (147 MB)
-// 39.6 us; one of 4071 keys 12.9 us, where launch, length, pages, keys, hand-over and join follow one another.
-// 3 waves a SIMD (168 registers) of 16 KB on their way each; at 2 the last case took 15.3, the second 48.
+// Bound by memory: 200 sequences up to 8192 keys (3.4 GB) 565 us, 6.0 TB/s (a large copy: 4.8); 48 up to 1500 (147 MB)
+// 39 us; one of 4071 keys 11.6 us, where launch, length, pages, keys, hand-over and join follow one another.
 struct PagedAttnArgs {
   const f16 *keys, *values;
   int64_t page_stride;
@@ -323,7 +322,7 @@ __device__ __forceinline__ float across_rows(float x, F f) {
 __device__ __forceinline__ float both_parts(float x) { return x + dpp_mov<0x128>(x); }
 
 template <typename T, int HD, int NT>
-__global__ __launch_bounds__(256, NT == 2 && HD == 128 ? 2 : HD == 64 && NT == 1 ? 4 : 3) void k_paged_attention(PagedAttnArgs a) {
+__global__ __launch_bounds__(256, 2) void k_paged_attention(PagedAttnArgs a) {
   constexpr int KC = HD / 32;  // 32-dim steps of a score
   constexpr int VD = HD / 16;  // dims of a value row a lane reads: 8 (16 bytes) or 4
   constexpr int HEADS = 8 * NT;
@@ -854,10 +853,11 @@ int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const
   const size_t part = static_cast<size_t>(a.group) * (hd + 2) * sizeof(float);
   const int64_t room = std::max<int64_t>(1, (int64_t{512} << 20) / static_cast<int64_t>(pairs * part));
   // Blocks of a sequence. `splits`: one for each CU where there are few sequences (8 x 1000 keys, 16 query and 8 KV
-  // heads: 12.5 us so, 15.4 with half of them; 8 x 4000, 32 and 8: 27 us, 31 with twice and 34 with four times as many),
-  // but 32 at most (one of 16000 keys, 14 and 2 heads: 19 us with 32 parts a head, 29 with 128). No block takes more
-  // than 1024 keys, so that ragged lengths even out. `grid`: what is launched for each row of the table, by its
-  // width alone; a large batch has 8 (64 rows of 200 keys in a table 32768 wide: 12 us, 41 with 32, most of them empty).
+  // heads: 11.8 us so, 14.6 with half of them; 8 x 4000, 32 and 8: 26.7 us, 28.1 with twice as many), but 32 at most (one
+  // of 16000 keys, 14 and 2 heads: 17.9 us with 32 parts a head, 19.4 with 63). No block takes more than 1024 keys, so
+  // that ragged lengths even out (512: 48 up to 1500 keys 34 us for 39, but 256 up to 1024 114 for 105). `grid`: what is
+  // launched for each row of the table, by its width alone; a large batch has 8 (64 rows of 200 keys in a table 32768
+  // wide: 11 us, 20 with 32, most of them empty).
   a.splits = static_cast<int>(std::min<int64_t>(32, (256 + pairs - 1) / pairs));
   a.grid = static_cast<int>(std::min({std::max<int64_t>(a.splits, (longest + soc::kAttentionMost - 1) / soc::kAttentionMost),
                                       std::max<int64_t>(8, 4096 / pairs), (longest + 127) / 128, room, int64_t{256}}));

@@ -38,7 +38,7 @@ SOC_HD int32_t checked_length(int32_t len, int32_t max_pages, int page_shift) {
 // Keys a block of the decode attention takes of a sequence of `len` > 0 keys: whole tiles of 128 (32 for each of its four
 // waves), so that the sequence gets at least `splits` blocks while it has tiles for them, and no block more than
 // kAttentionMost keys; but never more than `grid` blocks. More than 16 blocks take 256 keys at least: joining parts costs
-// more than shorter chunks save (one sequence of 4071 keys, 32 query and 8 KV heads: 12.8 us with 16 blocks, 14.1 with
+// more than shorter chunks save (one sequence of 4071 keys, 32 query and 8 KV heads: 11.6 us with 16 blocks, 12.4 with
 // 32).
 constexpr int32_t kAttentionMost = 1024;
 SOC_HD int32_t attention_chunk(int32_t len, int32_t splits, int32_t grid) {
