@@ -304,10 +304,12 @@ int soc_op_mul(soc_ctx* ctx, const float* a, const float* b, float* y, int32_t r
  *      A step is: soc_paged_plan (pages, slots and positions from the requests' lengths), then in each layer
  *      soc_paged_append (rotary positions; keys and values into their slots) and soc_paged_attention_decode, and at the
  *      end soc_logprobs of the chosen tokens. All calls check that each operand lies inside one device allocation of
- *      the context's device, are queued on the context stream without waiting, and hold their workspace in the context;
- *      an operand changed, freed or read by other means first waits for them (soc_ctx_synchronize). Operands of one call
- *      must not overlap except where its comment says so. What device memory holds (lengths, page ids, slots) is checked
- *      on the device: no value in it makes a kernel leave the operands' bounds. ---- */
+ *      the context's device, are queued on the context stream without waiting, and hold their workspace in the context
+ *      (a call that needs more of it than any before waits for the stream). What other streams do with an operand has to
+ *      be finished before the call; who reads, changes or frees an operand by other means first waits for the context
+ *      (soc_ctx_synchronize). Operands of one call must not overlap except where its comment says so. What device
+ *      memory holds (lengths, page ids, slots) is checked on the device: no value in it makes a kernel leave the
+ *      operands' bounds. ---- */
 /* Pairs rotated together: half (i, i + rotary_dim / 2), or interleaved (2 i, 2 i + 1). */
 enum { SOC_ROPE_HALF = 0, SOC_ROPE_INTERLEAVED = 1 };
 /* Long contexts: positions divided by `factor`; theta raised by factor^(d / (d - 2)); or the frequencies that turn
@@ -357,7 +359,8 @@ enum { SOC_PLAN_LENGTHS = 1, SOC_PLAN_CURSORS = 2, SOC_PLAN_PAGES = 4, SOC_PLAN_
  *     these are taken from the head and written to block_table row i (entries of table_stride elements a row, max_pages
  *     <= 2^18 of them used), requests in order, pages in order;
  *   shorter (finished: 0; or rolled back): its table's pages beyond the new length go to the ring's tail, requests in
- *     order, pages in order; the table row is left as it is.
+ *     order, pages in order; the table row is left as it is. (A page that several rows name would be given back by each
+ *     of them: who shares pages keeps their count.)
  * row_starts [n + 1]: exclusive sums of the rows. positions, slots [max_rows] (max_rows <= 2^22): each row's position
  * and slot (page * page_size + place; -1 where its page id is none of the cache); rows from the total on get position 0
  * and slot -1. cursors_out = the cursors after the step (may be cursors_in). Pages given back are first taken by a later
@@ -382,11 +385,12 @@ int soc_paged_append(soc_ctx* ctx, const soc_paged_cache* cache, const soc_rope*
 /* Attention of one token of each of n sequences over its cached positions [0, seq_lens[i]) (its own among them): q and
  * out (SOC_DTYPE_F32 or _F16) [n][q_heads * head_dim], rows q_stride and out_stride elements apart (out may be q with the
  * same stride); q_heads / kv_heads a whole number up to 16; scores times `scale` (finite; 0 means 1 / sqrt(head_dim)).
- * block_table: max_pages entries a row used, rows table_stride apart; pages may be shared by sequences. lse (nullable)
- * [n][q_heads]: log sum exp of the scores, to join with attention over other keys. A sequence of length 0 (or below)
- * gets zeros and lse -inf; one whose length goes beyond max_pages, or whose table names a page outside the cache within
- * its length, gets NaN. What lies in its last page behind its length is not used, whatever it holds. Where a NaN or an
- * infinity is among the queries, keys or values used, what it enters is the formula's result or NaN. */
+ * block_table: max_pages entries a row used (max_pages * page_size <= 2^30), rows table_stride apart; pages may be
+ * shared by sequences. lse (nullable) [n][q_heads]: log sum exp of the scores, to join with attention over other keys.
+ * A sequence of length 0 (or below) gets zeros and lse -inf; one whose length goes beyond max_pages, or whose table names
+ * a page outside the cache within its length, gets NaN. What lies in its last page behind its length is not used,
+ * whatever it holds. Where a NaN or an infinity is among the queries, keys or values used, what it enters is the
+ * formula's result or NaN. n * kv_heads <= 2^20. */
 int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const void* q, int64_t q_stride,
                                int32_t dtype, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
                                const int32_t* seq_lens, int32_t n, int32_t q_heads, float scale, void* out,

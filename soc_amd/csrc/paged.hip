@@ -381,7 +381,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedAttnArgs a) {
   const f16* keys = a.keys + (static_cast<int64_t>(g) << a.page_shift) * HD;
   const f16* values = a.values + (static_cast<int64_t>(g) << a.page_shift) * HD;
 
-  // keys count in unsigned words: those behind a length next to 2^31 do not wrap below it
+  // (key numbers are unsigned words: at most 2^30 keys and 2^14 behind them)
   auto within = [&](uint32_t key) { return min(key, static_cast<uint32_t>(len) - 1); };
   // lane l holds the page of half tile l % 2 of this wave's tile l / 2 (32 tiles ahead)
   bool lost = false;
@@ -809,8 +809,8 @@ int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const
   if (dtype != SOC_DTYPE_F32 && dtype != SOC_DTYPE_F16)
     return soc::fail(SOC_ERR_INVALID, "paged attention: dtype must be F32 or F16");
   if (n <= 0 || n > 65535) return soc::fail(SOC_ERR_INVALID, "paged attention: 1 to 65535 sequences");
-  if (max_pages <= 0 || static_cast<int64_t>(max_pages) * cache->page_size > INT32_MAX)
-    return soc::fail(SOC_ERR_INVALID, "paged attention: need max_pages > 0 and max_pages * page_size below 2^31");
+  if (max_pages <= 0 || static_cast<int64_t>(max_pages) * cache->page_size > (1 << 30))
+    return soc::fail(SOC_ERR_INVALID, "paged attention: need max_pages > 0 and max_pages * page_size up to 2^30");
   if (q_heads <= 0 || q_heads % cache->kv_heads != 0 || q_heads / cache->kv_heads > 16)
     return soc::fail(SOC_ERR_INVALID, "paged attention: query heads per KV head must be 1 to 16");
   if (!std::isfinite(scale)) return soc::fail(SOC_ERR_INVALID, "paged attention: scale must be finite");

@@ -61,7 +61,7 @@ int main() {
   }
   std::mt19937_64 rng(5);
   for (int i = 0; i < 200000; ++i) {
-    const int32_t len = 1 + static_cast<int32_t>((rng() >> 33) >> (rng() % 31)) % (INT32_MAX - 256);
+    const int32_t len = 1 + static_cast<int32_t>((rng() >> 33) >> (rng() % 31)) % (1 << 30);
     const int32_t splits = 1 + rng() % 200, grid = 1 + rng() % 300;
     const int64_t chunk = soc::attention_chunk(len, splits, grid), blocks = (len - 1) / chunk + 1;
     expect(chunk > 0 && chunk % 128 == 0, "a chunk is whole tiles");

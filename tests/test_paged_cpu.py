@@ -137,6 +137,8 @@ def test_attention_refusals():
     refused(attend(cache(), n=65536), "sequences")
     refused(attend(cache(), max_pages=0), "max_pages")
     refused(attend(cache(), max_pages=1 << 27), "max_pages")
+    refused(attend(cache(), max_pages=(1 << 26) + 1), "max_pages")
+    refused(attend(cache(), max_pages=1 << 26), "null context")
     refused(attend(cache(), q_heads=0), "query heads")
     refused(attend(cache(), q_heads=3), "query heads")
     refused(attend(cache(), q_heads=34), "query heads")
