@@ -301,7 +301,7 @@ struct PagedAttnArgs {
   int64_t out_stride;
   float* lse;
   bool wide_q;             // query rows are 32-byte aligned (16 in fp16): eight values a load
-  int splits, grid;        // attention_chunk
+  int splits, grid, most;  // attention_chunk
   float* part;             // [n][nkv][grid][group * (HD + 2)]: outputs, then maxima, then sums
   int* arrived;            // [n][nkv], zero between launches
 };
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedAttnArgs a) {
     if (lse != nullptr && tid < G) lse[tid] = len < 0 ? nan : -INFINITY;
     return;
   }
-  const int chunk = attention_chunk(len, a.splits, a.grid);
+  const int chunk = attention_chunk(len, a.splits, a.grid, a.most);
   const uint32_t c0 = static_cast<uint32_t>(s) * chunk;
   if (c0 >= static_cast<uint32_t>(len)) return;
   if (s != 0) load_queries();
@@ -854,12 +854,16 @@ int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const
   const int64_t room = std::max<int64_t>(1, (int64_t{512} << 20) / static_cast<int64_t>(pairs * part));
   // Blocks of a sequence. `splits`: one for each CU where there are few sequences (8 x 1000 keys, 16 query and 8 KV
   // heads: 11.8 us so, 14.6 with half of them; 8 x 4000, 32 and 8: 26.7 us, 28.1 with twice as many), but 32 at most (one
-  // of 16000 keys, 14 and 2 heads: 17.9 us with 32 parts a head, 19.4 with 63). No block takes more than 1024 keys, so
-  // that ragged lengths even out (512: 48 up to 1500 keys 34 us for 39, but 256 up to 1024 114 for 105). `grid`: what is
-  // launched for each row of the table, by its width alone; a large batch has 8 (64 rows of 200 keys in a table 32768
-  // wide: 11 us, 20 with 32, most of them empty).
+  // of 16000 keys, 14 and 2 heads: 17.9 us with 32 parts a head, 19.4 with 63).
+  // `most`: keys a block, so that ragged lengths even out: 1024 (512: 256 sequences up to 1500 keys, 32 and 8 heads,
+  // 162 us for 148); 2048 where whole sequences fill the 768 places for blocks twice over and a part is of four query
+  // heads or more, which cost most to prepare and join (256 up to 6000: 535 us for 551, all of 1500 248 for 272; but 128
+  // up to 1500 89 for 81, and 256 up to 1500 with 16 and 8 heads of 64 81 for 75).
+  // `grid`: what is launched for each row of the table, by its width alone; a large batch has 8 (64 rows of 200 keys in a
+  // table 32768 wide: 11 us, 20 with 32, most of them empty).
   a.splits = static_cast<int>(std::min<int64_t>(32, (256 + pairs - 1) / pairs));
-  a.grid = static_cast<int>(std::min({std::max<int64_t>(a.splits, (longest + soc::kAttentionMost - 1) / soc::kAttentionMost),
+  a.most = pairs >= 2 * 768 && a.group >= 4 ? 2048 : soc::kAttentionMost;
+  a.grid = static_cast<int>(std::min({((longest - 1) / a.most / a.splits + 1) * a.splits,
                                       std::max<int64_t>(8, 4096 / pairs), (longest + 127) / 128, room, int64_t{256}}));
   if (a.grid > 1) {
     SOC_TRY(soc::ensure_serve_ws(ctx, static_cast<size_t>(pairs) * a.grid * part, static_cast<size_t>(pairs)));

@@ -1,5 +1,6 @@
 // The index arithmetic of the paged cache (soc_amd/csrc/paged_math.h) on hostile values: whatever lengths, page ids,
 // slots and cursors device memory may hold, what comes out is in bounds or -1. Host only.
+#include <algorithm>
 #include <cstdint>
 #include <cstdio>
 #include <random>
@@ -62,12 +63,12 @@ int main() {
   std::mt19937_64 rng(5);
   for (int i = 0; i < 200000; ++i) {
     const int32_t len = 1 + static_cast<int32_t>((rng() >> 33) >> (rng() % 31)) % (1 << 30);
-    const int32_t splits = 1 + rng() % 200, grid = 1 + rng() % 300;
-    const int64_t chunk = soc::attention_chunk(len, splits, grid), blocks = (len - 1) / chunk + 1;
+    const int32_t splits = 1 + rng() % 200, grid = 1 + rng() % 300, most = 256 * (1 + rng() % 8);
+    const int64_t chunk = soc::attention_chunk(len, splits, grid, most), blocks = (len - 1) / chunk + 1;
     expect(chunk > 0 && chunk % 128 == 0, "a chunk is whole tiles");
     expect(blocks <= grid, "the grid holds a sequence's blocks");
     expect((blocks - 1) * chunk < len, "no block is empty");
-    if ((int64_t{len} - 1) / soc::kAttentionMost + 1 <= grid) expect(chunk <= soc::kAttentionMost, "no block takes more than it may");
+    if ((int64_t{len} - 1) / most + splits <= grid) expect(chunk <= std::max(most, soc::kAttentionMost), "no block takes more than it may");
     if (len > 128 * splits && splits <= grid) expect(blocks * 2 >= splits, "a long sequence gets its blocks");
   }
   for (int i = 0; i < 200000; ++i) {

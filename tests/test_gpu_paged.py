@@ -508,6 +508,14 @@ def test_attention_batches(gpu_ctx, lens):
     run_attention(gpu_ctx, "f32", lens, 8, 2, 128, 32)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attention_of_many_ragged_rows(gpu_ctx, dtype):
+    """Rows enough that blocks take up to 2048 keys: lengths around one block and two, and short ones among them."""
+    lens = np.random.default_rng(9).integers(0, 70, 1600)
+    lens[::100] = [2047, 2048, 2049, 4096, 4097, 1024, 1025, 0, 1, 1500, 2100, 3000, 768, 769, 128, 129]
+    run_attention(gpu_ctx, dtype, lens.tolist(), 5, 1, 64, 16, width=300)
+
+
 def test_attention_of_a_wide_table(gpu_ctx):
     """A table far wider than any sequence: lengths on the device decide, not the width."""
     a, la = run_attention(gpu_ctx, "f32", [40, 3000, 0, 17], 8, 2, 128, 16)
