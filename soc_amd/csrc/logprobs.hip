@@ -66,7 +66,7 @@ __device__ __forceinline__ uint64_t key_of(float x, int id) {
 // logit. Of the top n, each thread's largest token stands for its E: the n-th largest of those 256 keys is a threshold
 // that at most n threads reach, so at most n E tokens (64 of normal data) are candidates, and those rank each other. No
 // step depends on how many values are equal. The last block of a row to finish joins its chunks, in chunk order.
-// 777 rows of 151936 fp32 logits with top 8 take 99 us (4.75 TB/s, the rate of a large copy); one row 11.7 us with top
+// 777 rows of 151936 fp32 logits with top 8 take 98 us (4.8 TB/s, the rate of a large copy); one row 10.7 us with top
 // 20 and 5.1 us without: there the chain of reading, reducing, selecting, handing over and joining counts. At 32 fp32
 // logits a thread, 64 registers (8 waves a SIMD) are worth 5 % on many rows; in 16 bits they would spill.
 constexpr int kThreads = 256;
@@ -170,7 +170,8 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   __shared__ float red[3][4];
   __shared__ int count[4];
   __shared__ uint64_t threshold;
-  __shared__ int found, last, tied;
+  __shared__ int giver[kMaxTop];
+  __shared__ int found, givers, last, tied;
 
   const int64_t r = blockIdx.x / a.chunks;
   const int c = blockIdx.x % a.chunks;
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   for (int e = 1; e < E; ++e) best = fmaxf(best, v[e]);
   float m = wave_max(best);
   if (lane == 0) red[0][wid] = m;
-  if (tid == 0) found = 0;
+  if (tid == 0) found = givers = 0;
   __syncthreads();
   m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   // -inf alone sums to 0; NaN, or +inf less itself, makes the sums NaN
@@ -232,6 +233,7 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
     s += p;
     d = fmaf(p, fmaxf(u, -1000.0f), d);  // 2^-1000 is 0: a masked logit adds 0, not 0 times -inf
   }
+  auto place_of = [&](int thread, int e) { return lo + (thread + e / VW * kThreads) * VW + e % VW; };
   auto place = [&](int e) { return base + (e / VW) * kThreads * VW + e % VW; };  // the id of the thread's logit e
   // tokens before the given one: equal logits at lower ids, larger ones anywhere. What is not of the row is -inf here,
   // which is never counted: ids below 0 are taken as large ones
@@ -316,19 +318,33 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
     if (tid < n) first[tid] = 0;
     __syncthreads();
     const uint64_t t = max(threshold, uint64_t{1});
-    if (group[tid] >= t) {  // at most n threads
-      const float tv = value_of<T>(static_cast<uint32_t>(t >> 32));
+    const float tv = value_of<T>(static_cast<uint32_t>(t >> 32));
+    // the logits of the threads that reach it, at most n, are handed to all threads: E registers tested in place would be
+    // E copies of what follows, mostly skipped (one row top 20 11.6 us for 10.7, 777 fp16 rows 91 for 87)
+    float* handed = reinterpret_cast<float*>(keys);
+    if (group[tid] >= t) {
+      const int at = atomicAdd(&givers, 1);
+      giver[at] = tid;
 #pragma unroll
-      for (int q = 0; q < E; q += 4) {  // four at a time: a thread has a candidate or two among its logits
-        const float most = fmaxf(fmaxf(v[q], v[q + 1]), fmaxf(v[q + 2], v[q + 3]));
-        if (most < tv && s == s) continue;
+      for (int e = 0; e < E; ++e) handed[at * E + e] = v[e];
+    }
+    __syncthreads();
+    const int all = __builtin_amdgcn_readfirstlane(givers * E);
+    float y[kMaxTop * E / kThreads];
 #pragma unroll
-        for (int e = q; e < q + 4; ++e)
-          if (!(v[e] < tv)) {
-            const int id = place(e);
-            const uint64_t key = key_of<T>(v[e], id);
-            if (id >= 0 && id < a.vocab && key >= t) keys[atomicAdd(&found, 1)] = key;
-          }
+    for (int k = 0; k < kMaxTop * E / kThreads; ++k) {
+      if (k * kThreads >= all) break;
+      y[k] = handed[min(k * kThreads + tid, all - 1)];
+    }
+    __syncthreads();  // the keys take the logits' place
+#pragma unroll
+    for (int k = 0; k < kMaxTop * E / kThreads; ++k) {
+      if (k * kThreads >= all) break;
+      const int i = k * kThreads + tid;
+      if (i < all && !(y[k] < tv)) {
+        const int id = place_of(giver[i / E], i % E);
+        const uint64_t key = key_of<T>(y[k], id);
+        if (id >= 0 && id < a.vocab && key >= t) keys[atomicAdd(&found, 1)] = key;
       }
     }
     __syncthreads();
@@ -466,8 +482,8 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
   const bool aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && row_stride * size % 16 == 0;
   const int skip = aligned ? 0 : 16 / size - 1;  // the most that a row's chunks start before it
   auto chunks_of = [&](int each) { return (vocab + skip + soc::kThreads * each - 1) / (soc::kThreads * each); };
-  // chunks of 8192 logits (chunks of 16384: 777 rows of 151936 top 8 106 -> 94 us, 16 rows 13.3 -> 12.6); of 16384 where
-  // a row is one of them then, without a join (200 rows of 16384 top 5 11.8 -> 9.8 us), and beyond 2^18, for fewer joins
+  // chunks of 8192 logits (of 16384: 777 rows of 151936 top 8 102 us for 98, 64 in fp16 17.4 for 15.8); of 16384 where
+  // a row is one of them then, without a join (200 rows of 16384 top 5 9.4 us for 11.9), and beyond 2^18, for fewer joins
   const int each = (chunks_of(64) == 1 && chunks_of(32) > 1) || vocab > (1 << 18) ? 64 : 32;
   const int chunks = chunks_of(each);
   const size_t per_row = chunks > 1 ? chunks * (sizeof(soc::Part) + static_cast<size_t>(top_n) * 8) : 0;
