@@ -99,8 +99,9 @@ __device__ __forceinline__ void store_copy(const RopeUnit<T, W>& r, O* y) {
   store_vec<O, W>(y, x);
 }
 
-// Unit u, rotated, to y (O: another type where y is the cache's). Written as explicit fmaf, so that every width computes
-// the same bits.
+// Unit u, rotated, to y (O: another type where y is the cache's). Every width computes the same bits: the rotation is
+// written as explicit fmaf, and its fp32 results are materialised, since the compiler would otherwise fold the conversion
+// of some of a unit's values into their fma (v_fma_mixlo_f16, one rounding straight to fp16) and round the others twice.
 template <typename T, typename O, int W>
 __device__ __forceinline__ void store_unit(const RopeView& v, const f32x2* cs, const RopeUnit<T, W>& r, O* y, int u) {
   const int pair_units = v.rotary_dim / (2 * W);
@@ -121,6 +122,7 @@ __device__ __forceinline__ void store_unit(const RopeView& v, const f32x2* cs, c
     }
     p[i] = fmaf(a, t[0], -(b * t[1]));
     q[i] = fmaf(a, t[1], b * t[0]);
+    if constexpr (sizeof(O) == 2) __asm__ volatile("" : "+v"(p[i]), "+v"(q[i]));
   }
   if (v.interleaved) {
     float m[2 * W];
