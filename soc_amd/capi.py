@@ -194,6 +194,7 @@ def lib() -> C.CDLL:
         "soc_rope_destroy": (C.c_int, [P]),
         "soc_rope_apply": (C.c_int, [P, P, I64, P, I64, I32, I32, I32, P, I32]),
         "soc_paged_plan": (C.c_int, [P, I32, P, P, I32, P, I32, I64, P, I32, P, P, P, P, P, I32, P]),
+        "soc_paged_plan_step": (C.c_int, [P, I32, P, P, I32, P, I32, I64, P, I32, P, P, P, P, P, I32, P, P]),
         "soc_paged_append": (C.c_int, [P, P, P, P, I64, P, I64, P, I64, I32, P, I64, I32, I32, P, P]),
         "soc_paged_attention_decode": (C.c_int, [P, P, P, I64, I32, P, I64, I32, P, I32, I32, F32, P, I64, P]),
         "soc_logprobs": (C.c_int, [P, P, I32, I64, I32, I32, F32, P, P, P, P, I32, P, P]),
@@ -692,10 +693,12 @@ class PagedCache:
 
 def paged_plan(ctx: Context, n: int, old_lens: int, new_lens: int, page_size: int, block_table: int, max_pages: int,
                table_stride: int, free_ring: int, num_pages: int, cursors_in: int, cursors_out: int, row_starts: int,
-               positions: int, slots: int, max_rows: int, status: int) -> None:
-    check(lib().soc_paged_plan(ctx.h, n, old_lens, new_lens, page_size, block_table, max_pages, table_stride,
-                               free_ring, num_pages, cursors_in, cursors_out, row_starts, positions, slots, max_rows,
-                               status))
+               positions: int, slots: int, max_rows: int, status: int, step_lens: int | None = None) -> None:
+    """soc_paged_plan; with `step_lens` soc_paged_plan_step, whose lengths are safe to attend with before the status is
+    read."""
+    args = (ctx.h, n, old_lens, new_lens, page_size, block_table, max_pages, table_stride, free_ring, num_pages,
+            cursors_in, cursors_out, row_starts, positions, slots, max_rows, status)
+    check(lib().soc_paged_plan(*args) if step_lens is None else lib().soc_paged_plan_step(*args, step_lens))
 
 
 def paged_append(ctx: Context, cache: PagedCache, rope: "Rope | None", q: int | None, q_stride: int, k: int,

@@ -33,6 +33,7 @@ struct PlanArgs {
   int32_t *row_starts, *positions, *slots;
   int max_rows;
   int32_t* status;
+  int32_t* step_lens;  // nullptr: not asked for
   int* arrived;
 };
 
@@ -151,6 +152,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PlanArgs a) {
     a.slots[r] = slot;
   }
   for (int64_t i = gid; i <= a.n; i += stride) a.row_starts[i] = status == 0 ? rows[i] : 0;
+  if (a.step_lens != nullptr)
+    for (int64_t i = gid; i < a.n; i += stride) a.step_lens[i] = status == 0 ? a.after[i] : had[i];
   if (status == 0) {
     // entries at or behind the pages a request had are written, entries before them read: no thread reads what another
     // writes, and the ring's places from the tail on are not among those taken from the head (at most num_pages free)
@@ -696,27 +699,26 @@ int hip_status(hipError_t e, const char* what) {
   return e == hipSuccess ? SOC_OK : fail(SOC_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
 
-}  // namespace
-}  // namespace soc
-
-extern "C" {
-
-int soc_paged_plan(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const int32_t* new_lens, int32_t page_size,
-                   int32_t* block_table, int32_t max_pages, int64_t table_stride, int32_t* free_ring, int32_t num_pages,
-                   const int64_t* cursors_in, int64_t* cursors_out, int32_t* row_starts, int32_t* positions,
-                   int32_t* slots, int32_t max_rows, int32_t* status) {
-  SOC_API_BEGIN
-  if (n <= 0 || n > soc::kPlanMaxRequests) return soc::fail(SOC_ERR_INVALID, "paged plan: 1 to 4096 requests");
-  SOC_TRY(soc::check_page_size(page_size));
-  if (max_pages <= 0 || max_pages > soc::kPlanMaxPages)
-    return soc::fail(SOC_ERR_INVALID, "paged plan: max_pages must be 1 to 2^18");
-  if (max_rows <= 0 || max_rows > soc::kPlanMaxRows)
-    return soc::fail(SOC_ERR_INVALID, "paged plan: max_rows must be 1 to 2^22");
+// soc_paged_plan (step_lens: nullptr) and soc_paged_plan_step.
+int plan_step(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const int32_t* new_lens, int32_t page_size,
+              int32_t* block_table, int32_t max_pages, int64_t table_stride, int32_t* free_ring, int32_t num_pages,
+              const int64_t* cursors_in, int64_t* cursors_out, int32_t* row_starts, int32_t* positions, int32_t* slots,
+              int32_t max_rows, int32_t* status, int32_t* step_lens) {
+  if (n <= 0 || n > kPlanMaxRequests) return fail(SOC_ERR_INVALID, "paged plan: 1 to 4096 requests");
+  SOC_TRY(check_page_size(page_size));
+  if (max_pages <= 0 || max_pages > kPlanMaxPages)
+    return fail(SOC_ERR_INVALID, "paged plan: max_pages must be 1 to 2^18");
+  if (max_rows <= 0 || max_rows > kPlanMaxRows)
+    return fail(SOC_ERR_INVALID, "paged plan: max_rows must be 1 to 2^22");
   if (num_pages <= 0 || static_cast<int64_t>(num_pages) * page_size > INT32_MAX)
-    return soc::fail(SOC_ERR_INVALID, "paged plan: need num_pages > 0 and num_pages * page_size below 2^31");
-  if (ctx == nullptr) return soc::fail(SOC_ERR_INVALID, "null context");
-  soc::DeviceScope device(ctx);
-  soc::Operands operands(ctx);
+    return fail(SOC_ERR_INVALID, "paged plan: need num_pages > 0 and num_pages * page_size below 2^31");
+  if (step_lens != nullptr)  // another block may still read what one writes
+    for (const int32_t* lens : {old_lens, new_lens})
+      if (step_lens < lens + n && lens < step_lens + n)
+        return fail(SOC_ERR_INVALID, "paged plan: step_lens must not overlap old_lens or new_lens");
+  if (ctx == nullptr) return fail(SOC_ERR_INVALID, "null context");
+  DeviceScope device(ctx);
+  Operands operands(ctx);
   SOC_TRY(operands.array("paged plan old_lens", old_lens, n, 4));
   SOC_TRY(operands.array("paged plan new_lens", new_lens, n, 4));
   SOC_TRY(operands.rows("paged plan block_table", block_table, n, table_stride, max_pages, 4));
@@ -727,21 +729,45 @@ int soc_paged_plan(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const int32
   SOC_TRY(operands.array("paged plan positions", positions, max_rows, 4));
   SOC_TRY(operands.array("paged plan slots", slots, max_rows, 4));
   SOC_TRY(operands.array("paged plan status", status, 1, 4));
+  if (step_lens != nullptr) SOC_TRY(operands.array("paged plan step_lens", step_lens, n, 4));
   // a row a thread
-  const int blocks = std::min(256, std::max(1, (max_rows + soc::kPlanThreads - 1) / soc::kPlanThreads));
+  const int blocks = std::min(256, std::max(1, (max_rows + kPlanThreads - 1) / kPlanThreads));
   int* arrived = nullptr;
   if (blocks > 1 && cursors_out < cursors_in + 2 && cursors_in < cursors_out + 2) {
-    SOC_TRY(soc::ensure_serve_ws(ctx, 0, 1));
+    SOC_TRY(ensure_serve_ws(ctx, 0, 1));
     arrived = ctx->serve_counters;
   }
-  soc::PlanArgs a{n,         old_lens, new_lens,   block_table, max_pages,
-                  table_stride, free_ring, num_pages, soc::shift_of(page_size), cursors_in,
-                  cursors_out, row_starts, positions, slots, max_rows, status, arrived};
-  auto* kernel = n <= soc::kPlanThreads       ? soc::k_paged_plan<1>
-                 : n <= 4 * soc::kPlanThreads ? soc::k_paged_plan<4>
-                                              : soc::k_paged_plan<soc::kPlanMaxRequests / soc::kPlanThreads>;
-  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(soc::kPlanThreads), 0, ctx->stream, a);
-  return soc::hip_status(hipGetLastError(), "paged plan");
+  PlanArgs a{n, old_lens, new_lens, block_table, max_pages, table_stride, free_ring, num_pages, shift_of(page_size),
+             cursors_in, cursors_out, row_starts, positions, slots, max_rows, status, step_lens, arrived};
+  auto* kernel = n <= kPlanThreads       ? k_paged_plan<1>
+                 : n <= 4 * kPlanThreads ? k_paged_plan<4>
+                                         : k_paged_plan<kPlanMaxRequests / kPlanThreads>;
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kPlanThreads), 0, ctx->stream, a);
+  return hip_status(hipGetLastError(), "paged plan");
+}
+
+}  // namespace
+}  // namespace soc
+
+extern "C" {
+
+int soc_paged_plan(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const int32_t* new_lens, int32_t page_size,
+                   int32_t* block_table, int32_t max_pages, int64_t table_stride, int32_t* free_ring, int32_t num_pages,
+                   const int64_t* cursors_in, int64_t* cursors_out, int32_t* row_starts, int32_t* positions,
+                   int32_t* slots, int32_t max_rows, int32_t* status) {
+  SOC_API_BEGIN
+  return soc::plan_step(ctx, n, old_lens, new_lens, page_size, block_table, max_pages, table_stride, free_ring, num_pages,
+                        cursors_in, cursors_out, row_starts, positions, slots, max_rows, status, nullptr);
+  SOC_API_END
+}
+
+int soc_paged_plan_step(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const int32_t* new_lens, int32_t page_size,
+                        int32_t* block_table, int32_t max_pages, int64_t table_stride, int32_t* free_ring,
+                        int32_t num_pages, const int64_t* cursors_in, int64_t* cursors_out, int32_t* row_starts,
+                        int32_t* positions, int32_t* slots, int32_t max_rows, int32_t* status, int32_t* step_lens) {
+  SOC_API_BEGIN
+  return soc::plan_step(ctx, n, old_lens, new_lens, page_size, block_table, max_pages, table_stride, free_ring, num_pages,
+                        cursors_in, cursors_out, row_starts, positions, slots, max_rows, status, step_lens);
   SOC_API_END
 }
 
