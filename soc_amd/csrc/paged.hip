@@ -441,7 +441,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedAttnArgs a) {
     const int exponent = static_cast<int>(__float_as_uint(big) >> 23);
     const int e = big > 0.0f && exponent < 255 ? min(140 - exponent, 126) : 0;
     const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-    to_log2[t] = a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    // the power of two first: scale times log2(e) alone may pass fp32
+    to_log2[t] = a.scale * __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * kLog2e;
 #pragma unroll
     for (int c = 0; c < KC; ++c)
 #pragma unroll

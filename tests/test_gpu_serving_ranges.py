@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 from tests.test_gpu_logprobs import run as run_logprobs, verify as verify_logprobs
+from tests.test_gpu_paged import run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -23,3 +24,10 @@ def test_logprobs_of_logits_further_apart_than_fp32_reaches(gpu_ctx, vocab, t):
     verify_logprobs(got[0], t, tokens, 64, *got[1:])
     got = run_logprobs(gpu_ctx, x, "f32", t, tokens, 0)
     verify_logprobs(got[0], t, tokens, 0, *got[1:])
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38, 1e-38])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_scales_at_the_ends_of_fp32(gpu_ctx, scale, hd):
+    """A scale times log2(e) may pass fp32 where the scores do not."""
+    run_attention(gpu_ctx, "f32", [70, 900, 5], 8, 2, hd, 16, scale=scale, q_scale=1e-38 if abs(scale) > 1 else 1e37)
