@@ -704,6 +704,8 @@ def paged_plan(ctx: Context, n: int, old_lens: int, new_lens: int, page_size: in
 def paged_append(ctx: Context, cache: PagedCache, rope: "Rope | None", q: int | None, q_stride: int, k: int,
                  k_stride: int, v: int, v_stride: int, dtype: str, q_out: int | None, q_out_stride: int, rows: int,
                  q_heads: int, positions: int | None, slots: int) -> None:
+    if rope is not None and rope.h is None:  # a null handle would mean keys without rotation
+        raise SocError(SOC_ERR_INVALID, "paged append: the rope is closed")
     check(lib().soc_paged_append(ctx.h, cache.ref, rope.h if rope is not None else None, q, q_stride, k, k_stride, v,
                                  v_stride, DTYPES[dtype], q_out, q_out_stride, rows, q_heads, positions, slots))
 
