@@ -332,15 +332,17 @@ typedef struct soc_rope soc_rope;
 int soc_rope_create(soc_ctx* ctx, const soc_rope_spec* spec, soc_rope** out);
 int soc_rope_destroy(soc_rope* rope);
 /* Rotates `heads` heads of `rows` rows x -> y (SOC_DTYPE_F32 or _F16; rows x_stride and y_stride elements apart, each at
- * least heads * head_dim): row r at position positions[r] (device memory, any int32), or position_offset + r where
- * positions is NULL. The angles are formed in 64 bits. Dims from rotary_dim on are copied. y may be x with the same
+ * least heads * head_dim, which is at most 2^30): row r at position positions[r] (device memory, any int32), or
+ * position_offset + r where positions is NULL. The angles are formed in 64 bits, rotated in 32; fp16 results are the fp32
+ * ones rounded to nearest, at every alignment and stride. Dims from rotary_dim on are copied. y may be x with the same
  * stride. */
 int soc_rope_apply(const soc_rope* rope, const void* x, int64_t x_stride, void* y, int64_t y_stride, int32_t dtype,
                    int32_t rows, int32_t heads, const int32_t* positions, int32_t position_offset);
 /* One layer's pages: fp16; dim i of the position at place t of page p and KV head h is element
  * p * page_stride + (h * page_size + t) * head_dim + i of `keys` and of `values`. page_stride: 0, or at least
  * kv_heads * page_size * head_dim and a multiple of 8 (pools that interleave layers, or keys with values). page_size:
- * 16, 32, 64, 128 or 256; head_dim: 64 or 128; num_pages * page_size < 2^31; keys and values 16-byte aligned. */
+ * 16, 32, 64, 128 or 256; head_dim: 64 or 128; kv_heads: 1 to 1024; num_pages * page_size < 2^31; keys and values 16-byte
+ * aligned. */
 typedef struct soc_paged_cache {
   void* keys;
   void* values;
@@ -385,7 +387,8 @@ int soc_paged_plan_step(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const 
 /* A step's new rows into the cache: row r's kv_heads keys, rotated at positions[r], and values go to slots[r], rounded
  * to fp16 to nearest; its q_heads queries, rotated, to q_out. q, k, v (SOC_DTYPE_F32 or _F16) and q_out (same type):
  * rows q_stride, k_stride, v_stride, q_out_stride elements apart, so that the three may be parts of one fused
- * projection; q_out may be q with the same stride. q_heads may be 0 (q and q_out unused). rope: of the cache's head_dim;
+ * projection; q_out may be q with the same stride. q_heads: up to 65536, or 0 (q and q_out unused). Values rotated and
+ * rounded as by soc_rope_apply; a model that norms its heads does so before (soc_op_rmsnorm). rope: of the cache's head_dim;
  * NULL stores keys unrotated (then q_heads must be 0 and positions is unused). A row whose slot is negative or outside
  * the cache is skipped: nothing of it is stored, its q_out row is left as it is. Slots of one call must differ. */
 int soc_paged_append(soc_ctx* ctx, const soc_paged_cache* cache, const soc_rope* rope, const void* q, int64_t q_stride,
@@ -401,7 +404,9 @@ int soc_paged_append(soc_ctx* ctx, const soc_paged_cache* cache, const soc_rope*
  * a page outside the cache within its length, gets NaN. A page of the cache that is another sequence's by now is read as if
  * it were its own: lengths are those that a plan gave (soc_paged_plan_step). What lies in its last page behind its length
  * is not used, whatever it holds. Where a NaN or an infinity is among the queries, keys or values used, what it enters is
- * the formula's result or NaN. n * kv_heads <= 2^20. */
+ * the formula's result or NaN; a score beyond fp32's range is such an infinity. n <= 65535, n * kv_heads <= 2^20.
+ * A sequence's bits follow from its own query, keys, values and length, and from n, the head counts, max_pages and
+ * page_size, by which its keys are split over blocks; not from the other sequences' lengths or contents. */
 int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const void* q, int64_t q_stride,
                                int32_t dtype, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
                                const int32_t* seq_lens, int32_t n, int32_t q_heads, float scale, void* out,
@@ -415,7 +420,8 @@ int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const
  *   top_ids, top_logprobs [rows][top_n] (0 <= top_n <= min(64, vocab); NULL at 0): the tokens of the largest logits in
  *     order, equal logits by lowest id.
  * -inf masks a token: log probability -inf, no part in the entropy. A row of nothing but -inf has log probabilities -inf
- * and entropy 0. A row that holds a NaN or +inf has log probabilities and entropy NaN; NaNs are ordered above +inf. */
+ * and entropy 0. A row that holds a NaN or +inf has log probabilities and entropy NaN; NaNs are ordered above +inf.
+ * A row's bits follow from its logits, the vocabulary and the rows' alignment, not from the other rows. */
 int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab,
                  float temperature, const int32_t* tokens, float* logprobs, int32_t* ranks, float* entropy,
                  int32_t top_n, int32_t* top_ids, float* top_logprobs);
