@@ -366,20 +366,20 @@ enum { SOC_PLAN_LENGTHS = 1, SOC_PLAN_CURSORS = 2, SOC_PLAN_PAGES = 4, SOC_PLAN_
  * row_starts [n + 1]: exclusive sums of the rows. positions, slots [max_rows] (max_rows <= 2^22): each row's position
  * and slot (page * page_size + place; -1 where its page id is none of the cache); rows from the total on get position 0
  * and slot -1. cursors_out = the cursors after the step (may be cursors_in). Pages given back are first taken by a later
- * plan. *status = 0; or bits, and then nothing is taken or given: row_starts and positions are 0, slots -1, cursors_out =
- * cursors_in, table and ring untouched (for what is queued behind it, see soc_paged_plan_step). The bits: LENGTHS, a
- * length is negative or beyond max_pages; CURSORS, the ring would hold fewer than 0 or more than num_pages entries; PAGES,
- * more pages needed than free; ROWS, more than max_rows rows. The result does not depend on timing: equal inputs give
- * equal outputs. */
+ * plan. *status = 0; or bits, and then nothing is taken or given: row_starts and positions are 0, slots -1, cursors_out
+ * = cursors_in, table and ring untouched (for what is queued behind it, see soc_paged_plan_step). The bits: LENGTHS, a
+ * length is negative or beyond max_pages; CURSORS, the ring would hold fewer than 0 or more than num_pages entries;
+ * PAGES, more pages needed than free; ROWS, more than max_rows rows. The result does not depend on timing: equal inputs
+ * give equal outputs. */
 int soc_paged_plan(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const int32_t* new_lens, int32_t page_size,
                    int32_t* block_table, int32_t max_pages, int64_t table_stride, int32_t* free_ring, int32_t num_pages,
                    const int64_t* cursors_in, int64_t* cursors_out, int32_t* row_starts, int32_t* positions,
                    int32_t* slots, int32_t max_rows, int32_t* status);
-/* The same, and step_lens [n] (nullable): the lengths that hold after the step, new_lens where status is 0, else old_lens.
- * Attention that is queued behind a plan whose status the host has not read takes these. With new_lens it would, after a
- * refused step, read table entries behind the pages a request holds, and those may name pages that are others' by now:
- * keys and values of another request, with no sign of it. (What follows from a refused step is discarded either way.)
- * step_lens must not overlap old_lens or new_lens. */
+/* The same, and step_lens [n] (nullable): the lengths that hold after the step, new_lens where status is 0, else
+ * old_lens. Attention that is queued behind a plan whose status the host has not read takes these. With new_lens it
+ * would, after a refused step, read table entries behind the pages a request holds, and those may name pages that are
+ * others' by now: keys and values of another request, with no sign of it. (What follows from a refused step is
+ * discarded either way.) step_lens must not overlap old_lens or new_lens. */
 int soc_paged_plan_step(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const int32_t* new_lens, int32_t page_size,
                         int32_t* block_table, int32_t max_pages, int64_t table_stride, int32_t* free_ring,
                         int32_t num_pages, const int64_t* cursors_in, int64_t* cursors_out, int32_t* row_starts,
@@ -387,10 +387,11 @@ int soc_paged_plan_step(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const 
 /* A step's new rows into the cache: row r's kv_heads keys, rotated at positions[r], and values go to slots[r], rounded
  * to fp16 to nearest; its q_heads queries, rotated, to q_out. q, k, v (SOC_DTYPE_F32 or _F16) and q_out (same type):
  * rows q_stride, k_stride, v_stride, q_out_stride elements apart, so that the three may be parts of one fused
- * projection; q_out may be q with the same stride. q_heads: up to 65536, or 0 (q and q_out unused). Values rotated and
- * rounded as by soc_rope_apply; a model that norms its heads does so before (soc_op_rmsnorm). rope: of the cache's head_dim;
- * NULL stores keys unrotated (then q_heads must be 0 and positions is unused). A row whose slot is negative or outside
- * the cache is skipped: nothing of it is stored, its q_out row is left as it is. Slots of one call must differ. */
+ * projection; q_out may be q with the same stride. q_heads: up to 65536, or 0 (q and q_out unused). Values are rotated
+ * and rounded as by soc_rope_apply; a model that norms its heads does so before (soc_op_rmsnorm). rope: of the cache's
+ * head_dim; NULL stores keys unrotated (then q_heads must be 0 and positions is unused). A row whose slot is negative
+ * or outside the cache is skipped: nothing of it is stored, its q_out row is left as it is. Slots of one call must
+ * differ. */
 int soc_paged_append(soc_ctx* ctx, const soc_paged_cache* cache, const soc_rope* rope, const void* q, int64_t q_stride,
                      const void* k, int64_t k_stride, const void* v, int64_t v_stride, int32_t dtype, void* q_out,
                      int64_t q_out_stride, int32_t rows, int32_t q_heads, const int32_t* positions,
@@ -400,11 +401,12 @@ int soc_paged_append(soc_ctx* ctx, const soc_paged_cache* cache, const soc_rope*
  * same stride); q_heads / kv_heads a whole number up to 16; scores times `scale` (finite; 0 means 1 / sqrt(head_dim)).
  * block_table: max_pages entries a row used (max_pages * page_size <= 2^30), rows table_stride apart; pages may be
  * shared by sequences. lse (nullable) [n][q_heads]: log sum exp of the scores, to join with attention over other keys.
- * A sequence of length 0 (or below) gets zeros and lse -inf; one whose length goes beyond max_pages, or whose table names
- * a page outside the cache within its length, gets NaN. A page of the cache that is another sequence's by now is read as if
- * it were its own: lengths are those that a plan gave (soc_paged_plan_step). What lies in its last page behind its length
- * is not used, whatever it holds. Where a NaN or an infinity is among the queries, keys or values used, what it enters is
- * the formula's result or NaN; a score beyond fp32's range is such an infinity. n <= 65535, n * kv_heads <= 2^20.
+ * A sequence of length 0 (or below) gets zeros and lse -inf; one whose length goes beyond max_pages, or whose table
+ * names a page outside the cache within its length, gets NaN. A page of the cache that is another sequence's by now is
+ * read as if it were its own: lengths are those that a plan gave (soc_paged_plan_step). What lies in its last page
+ * behind its length is not used, whatever it holds. Where a NaN or an infinity is among the queries, keys or values
+ * used, what it enters is the formula's result or NaN; a score beyond fp32's range is such an infinity. n <= 65535
+ * and n * kv_heads <= 2^20.
  * A sequence's bits follow from its own query, keys, values and length, and from n, the head counts, max_pages and
  * page_size, by which its keys are split over blocks; not from the other sequences' lengths or contents. */
 int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const void* q, int64_t q_stride,

@@ -5,8 +5,8 @@
 //   log p_i = d_i - log S,  entropy = log S - D / S.
 // Differences are taken before they are scaled, so that nothing of the logits' common size enters the sums. Two fp32
 // logits can be further apart than fp32 reaches. A temperature above 1 could bring that back into its range, so from 1 on
-// log p takes halves of the logits, subtracted in one fma, and twice the scale: the same bits otherwise. In the sums such a
-// difference is -inf, whose exponential is the 0 that it has at temperatures up to 2^120 anyway (d below -256); beyond
+// log p takes halves of the logits, subtracted in one fma, and twice the scale: the same bits otherwise. In the sums such
+// a difference is -inf, whose exponential is the 0 that it has at temperatures up to 2^120 anyway (d below -256); beyond
 // them the sums take halves too. Always taking them costs fp32 rows 2.5 % (777 x 151936 97.6 us for 95.2).
 #include <algorithm>
 #include <cmath>
@@ -67,14 +67,15 @@ __device__ __forceinline__ uint64_t key_of(float x, int id) {
 }
 
 // One block per chunk of a row: 256 threads with E logits each in registers, read once in 16-byte loads, all requested
-// before the first is used. The chunk's
-// maximum comes first, so that every exponential is taken once; the count of tokens before the given one is a ballot per
-// logit. Of the top n, each thread's largest token stands for its E: the n-th largest of those 256 keys is a threshold
-// that at most n threads reach, so at most n E tokens (64 of normal data) are candidates, and those rank each other. No
-// step depends on how many values are equal. The last block of a row to finish joins its chunks, in chunk order.
-// 777 rows of 151936 fp32 logits with top 8 take 98 us (4.8 TB/s, the rate of a large copy); one row 10.7 us with top
-// 20 and 5.1 us without: there the chain of reading, reducing, selecting, handing over and joining counts. At 32 fp32
-// logits a thread, 64 registers (8 waves a SIMD) are worth 5 % on many rows; in 16 bits they would spill.
+// before the first is used. The chunk's maximum comes first, so that every exponential is taken once; each thread counts
+// its tokens before the given one, and one sum over the block follows. Of the top n, each thread's largest token stands
+// for its E: the n-th largest of those 256 keys is a threshold that at most n threads reach, so at most n E tokens (64 of
+// normal data) are candidates, and those rank each other. No step depends on how many values are equal. The last block of
+// a row to finish joins its chunks, in chunk order.
+// 777 rows of 151936 fp32 logits with top 8 take 96 us (4.9 TB/s; 87 us without alternatives, 5.4 TB/s). The same in fp16
+// takes 87 us, so there the instructions a logit count, not memory. One row takes 10.7 us with top 20 and 5.3 without:
+// the chain of reading, reducing, selecting, handing over and joining. At 32 fp32 logits a thread, 64 registers (8 waves
+// a SIMD) are worth 5 % on many rows; in 16 bits they would spill.
 constexpr int kThreads = 256;
 // Keys in LDS: the candidates of a chunk (top_n threads of E tokens); then the top_n of every chunk that one block joins,
 // and those of them at the threshold.

@@ -16,8 +16,9 @@ namespace {
 // One launch. Every block forms the same exclusive sums over the requests (rows, pages taken, pages given back) in LDS,
 // so that no block waits for another, and then finds the request of each of its rows and pages by bisection. The sums
 // are over at most 4096 lengths, read from L2; a second launch for them alone would cost more than repeating them. Bound
-// by latency (lengths, scan, bisection, table, store): 64 requests of one row 5.7 us a call, 4.2 of them the kernel's;
-// 1000 requests with 32768 rows 7.0, 6.9.
+// by latency (lengths, scan, bisection, table, store): 64 requests of one row 5.8 us a call, 4.3 of them the kernel's;
+// 1000 requests with 32768 rows 7.0. Beyond 1024 requests a thread holds sixteen, in 452 registers: 2000 with a row each
+// take 15.1 us, 4096 with 32000 rows 19.
 constexpr int kPlanThreads = 256;
 
 struct PlanArgs {
@@ -200,7 +201,7 @@ struct AppendArgs {
 // One row a block, or `parts` blocks where there are few rows: the units (rope.h) of the query heads, of the key heads,
 // then the value heads' W values each. The first unit is requested before slot and angles are known; a row without a
 // slot ends there. Bound by memory: 2531 rows of 16 query and 8 KV heads fp32 (72.6 MB) 13.1 us, 5.5 TB/s; 48 rows
-// of 32 and 8 by the launch: 5.5 us a call, 3.4 of them the kernel's (4.5 with one block a row).
+// of 32 and 8 by the launch: 5.7 us a call, 3.4 of them the kernel's (4.5 with one block a row). In fp16 8.9 and 5.6 us.
 template <typename T, int W>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
   __shared__ f32x2 cs[64];  // head_dim <= 128
@@ -288,8 +289,11 @@ hipError_t launch_paged_append(AppendArgs a, int64_t rows, hipStream_t s) {
 //           the columns as the queries are, and scaled by 2^14 so that small weights stay normal fp16 numbers.
 // Keys behind the sequence's end are read as its last key and get weight 0: what memory holds there is never used.
 //
-// Bound by memory: 200 sequences up to 8192 keys (3.4 GB) 565 us, 6.0 TB/s (a large copy: 4.8); 48 up to 1500 (147 MB)
-// 39 us; one of 4071 keys 11.6 us, where launch, length, pages, keys, hand-over and join follow one another.
+// Bound by memory: 200 sequences up to 8192 keys, 32 query and 8 KV heads (3.4 GB), 550 us, 6.2 TB/s (head_dim 64 285 us,
+// 6.0); 48 up to 1500 (147 MB) 38 us; one of 4071 keys 11.5 us, where launch, length, pages, keys, hand-over and join
+// follow one another. Groups of 9 to 16 heads take two tiles of columns in up to 221 registers, two blocks a CU: 48 query
+// and 4 KV heads, 200 sequences up to 8192 keys (1.7 GB) 358 us, 4.8 TB/s (32 and 4: 338, 5.0); one of 4071 keys 15.4
+// (32 and 4: 12.6).
 struct PagedAttnArgs {
   const f16 *keys, *values;
   int64_t page_stride;
@@ -883,11 +887,13 @@ int soc_paged_attention_decode(soc_ctx* ctx, const soc_paged_cache* cache, const
   // heads: 11.8 us so, 14.6 with half of them; 8 x 4000, 32 and 8: 26.7 us, 28.1 with twice as many), but 32 at most (one
   // of 16000 keys, 14 and 2 heads: 17.9 us with 32 parts a head, 19.4 with 63).
   // `most`: keys a block, so that ragged lengths even out: 1024 (512: 256 sequences up to 1500 keys, 32 and 8 heads,
-  // 162 us for 148); 2048 where whole sequences fill the 768 places for blocks twice over and a part is of four query
-  // heads or more, which cost most to prepare and join (256 up to 6000: 535 us for 551, all of 1500 248 for 272; but 128
-  // up to 1500 89 for 81, and 256 up to 1500 with 16 and 8 heads of 64 81 for 75).
+  // 162 us for 148); 2048 where whole sequences fill 768 places for blocks twice over (three a CU: head_dim 128 and up to
+  // 8 heads a group; the other kernels have two to four a CU, not measured apart) and a part is of four query heads or
+  // more, which cost most to prepare and join (256 up to 6000: 535 us for 551, all of 1500 248 for 272; but 128 up to 1500
+  // 89 for 81, and 256 up to 1500 with 16 and 8 heads of 64 81 for 75).
   // `grid`: what is launched for each row of the table, by its width alone; a large batch has 8 (64 rows of 200 keys in a
-  // table 32768 wide: 11 us, 20 with 32, most of them empty).
+  // table 32768 wide: 11 us, 20 with 32, most of them empty). The price: one long sequence among many short ones has 8
+  // blocks too, of whatever length (one of 131072 keys among 64 of 200, 32 and 8 heads: 448 us; alone 95).
   a.splits = static_cast<int>(std::min<int64_t>(32, (256 + pairs - 1) / pairs));
   a.most = pairs >= 2 * 768 && a.group >= 4 ? 2048 : soc::kAttentionMost;
   a.grid = static_cast<int>(std::min({((longest - 1) / a.most / a.splits + 1) * a.splits,

@@ -41,6 +41,8 @@ SOC_HD int32_t checked_length(int32_t len, int32_t max_pages, int page_shift) {
 // blocks. The multiple, because `splits` fills the card once: 16 sequences of 3000 keys, 32 query and 8 KV heads, take
 // 38 us with four blocks each, 43 with three. More than 16 blocks take 256 keys at least: joining parts costs more than
 // shorter chunks save (one sequence of 4071 keys, 32 and 8 heads: 11.6 us with 16 blocks, 12.4 with 32).
+// Where `grid` is the least of these bounds (8 in a large batch), a long sequence's blocks take as many keys as that
+// leaves them, beyond `most`.
 constexpr int32_t kAttentionMost = 1024;
 SOC_HD int32_t attention_chunk(int32_t len, int32_t splits, int32_t grid, int32_t most) {
   int32_t want = splits;

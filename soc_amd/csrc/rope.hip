@@ -15,8 +15,9 @@ namespace {
 
 // One row a block, or `parts` blocks where there are few rows. The first unit's values are requested before the angles are
 // formed: cosines and sines (one double product, one sincospi a pair) serve all heads of the row from LDS.
-// Bound by memory: 4093 rows x 16 heads of 128 fp16 values (33.5 MB) 7.9 us, 4.2 TB/s; 64 rows x 32 heads fp32 by the
-// launch: 5.2 us a call, 3.0 of them the kernel's.
+// Bound by memory: 4093 rows x 16 heads of 128 fp16 values (33.5 MB) 8.2 us, 4.1 TB/s; 64 rows x 32 heads fp32 by the
+// launch: 5.2 us a call, 3.0 of them the kernel's. One by one (pairs not in fours, or rows not 16-byte aligned) costs 1.5
+// to 3 times that: 8000 rows x 40 heads of 80, 20 of them rotated, 48 us in fp32 and 46 in fp16, all 80 rotated 31 and 17.
 template <typename T, int W>
 __global__ __launch_bounds__(256) void k_rope_rows(RopeView v, const T* x, int64_t x_stride, T* y, int64_t y_stride,
                                                    int heads, const int32_t* __restrict__ positions, uint32_t offset,
