@@ -379,7 +379,9 @@ int soc_paged_plan(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const int32
  * old_lens. Attention that is queued behind a plan whose status the host has not read takes these. With new_lens it
  * would, after a refused step, read table entries behind the pages a request holds, and those may name pages that are
  * others' by now: keys and values of another request, with no sign of it. (What follows from a refused step is
- * discarded either way.) step_lens must not overlap old_lens or new_lens. */
+ * discarded either way.) A later plan's old_lens must be lengths that hold: before it is queued the host reads the status,
+ * or knows from the ring's count, which it can follow, that the step was done. step_lens must not overlap old_lens or
+ * new_lens. */
 int soc_paged_plan_step(soc_ctx* ctx, int32_t n, const int32_t* old_lens, const int32_t* new_lens, int32_t page_size,
                         int32_t* block_table, int32_t max_pages, int64_t table_stride, int32_t* free_ring,
                         int32_t num_pages, const int64_t* cursors_in, int64_t* cursors_out, int32_t* row_starts,
