@@ -430,6 +430,53 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
                  float temperature, const int32_t* tokens, float* logprobs, int32_t* ranks, float* entropy,
                  int32_t top_n, int32_t* top_ids, float* top_logprobs);
 
+/* ---- rows that go on from other rows: beams of a search, samples of one prompt, prompts that begin alike. Full pages may be
+ *      named by any number of rows; a page that is partly filled belongs to one. A step is: soc_beam_select (or any choice
+ *      of parents), soc_paged_fork (the table rows that follow the choice), soc_paged_copy (the pages that two rows would
+ *      otherwise write, all layers), then a step as above from the lengths that the fork gives, its attention by
+ *      soc_paged_attention_shared. Rows that share pages end, or get shorter than what they share, by a fork and not by a
+ *      plan (which gives back each row's pages, whoever else names them). What holds for the calls above holds here. ---- */
+/* The table after row i has gone on from row parents[i] (-1: it ends) with its first keep[i] positions (keep NULL: all that
+ * old_lens[parents[i]] says); 1 <= n <= 4096 rows, and they are all that hold pages: new_table row i names its parent's
+ * pages, but where keep[i] ends inside a page, that page is new, taken from the ring's head in order of the rows, and to be
+ * copied from the parent's. The exception: the parent's own partly filled last page goes on in the first row of those
+ * children that need it. (A page that the parent has filled is copied, even if no other row names it.)
+ *   copies [n][3], of which *copy_count are written: (the page copied from, to, positions), as soc_paged_copy takes them.
+ *     Entries behind them are left as they are.
+ *   Pages that a row of block_table names within old_lens, and no row of new_table, go to the ring's tail, once each: rows in
+ *     order, pages in order, each page in the place of the last row that lost it.
+ *   new_lens [n]: keep, or 0 where parents[i] is -1. next_lens [n] (nullable): one more where the row goes on, else 0 (what a
+ *     plan takes as new_lens in a step of single tokens).
+ * new_table must not overlap block_table (entries behind a row's pages are left as they are), new_lens and next_lens not
+ * parents, keep or old_lens; cursors_out may be cursors_in. max_pages <= 2^18. *status = 0; or bits, and then new_table names
+ * what block_table does, new_lens and next_lens are old_lens, *copy_count is 0, ring and cursors as they were:
+ * SOC_PLAN_LENGTHS, a parent, length or keep out of range (keep beyond its parent's length); SOC_PLAN_CURSORS;
+ * SOC_PLAN_PAGES, more copies than free pages. Page ids that are none of the cache are passed on and never freed. Equal
+ * inputs give equal outputs. */
+int soc_paged_fork(soc_ctx* ctx, int32_t n, const int32_t* parents, const int32_t* keep, const int32_t* old_lens,
+                   int32_t page_size, const int32_t* block_table, int32_t* new_table, int32_t max_pages,
+                   int64_t table_stride, int32_t* free_ring, int32_t num_pages, const int64_t* cursors_in,
+                   int64_t* cursors_out, int32_t* new_lens, int32_t* next_lens, int32_t* copies, int32_t* copy_count,
+                   int32_t* status);
+/* Copies pages in `layers` caches of one shape (num_pages, page_size, kv_heads, head_dim; `caches`: host memory): for each
+ * of *move_count moves (NULL: max_moves; more than max_moves: those) [from, to, positions] the first `positions` places of
+ * page `from`, keys and values of all heads, to page `to`. A move with a page outside the cache, or to itself, is skipped;
+ * positions count up to page_size. No page that a move writes may be another's source or target. */
+int soc_paged_copy(soc_ctx* ctx, const soc_paged_cache* caches, int32_t layers, const int32_t* moves,
+                   const int32_t* move_count, int32_t max_moves);
+/* Brings the pages in use (those of the pool that are not free) to its front: the k-th highest of them moves to the k-th
+ * lowest free page, for as long as that is a lower one, at most max_moves times. moves [max_moves][3], of which *move_count
+ * are written: (from, to, page_size), as soc_paged_copy takes them, which has to follow before the cache is used.
+ * new_table: the n rows' entries within lens, moved pages by their new ids (entries behind them left as they are). new_ring:
+ * the free pages at the same places head .. tail - 1, lowest first; the cursors hold on. With enough moves the first
+ * num_pages - (tail - head) pages are those in use. new_table may be block_table, new_ring free_ring; else they must not
+ * overlap. num_pages <= 2^20. *status = 0; or bits, and then nothing moves: SOC_PLAN_LENGTHS, a length out of range;
+ * SOC_PLAN_CURSORS, cursors out of range, or free entries that are no page of the pool or the same one twice. */
+int soc_paged_compact(soc_ctx* ctx, int32_t n, const int32_t* lens, int32_t page_size, const int32_t* block_table,
+                      int32_t* new_table, int32_t max_pages, int64_t table_stride, const int32_t* free_ring,
+                      int32_t* new_ring, int32_t num_pages, const int64_t* cursors, int32_t* moves, int32_t max_moves,
+                      int32_t* move_count, int32_t* status);
+
 /* ---- seeded synthetic data (this project's generator; the reference has none) ---- */
 int soc_synth_normal_f16(uint64_t seed, const char* name, float sigma, int64_t offset, int64_t n, uint16_t* out);
 int soc_synth_uniform_f16(uint64_t seed, const char* name, float lo, float hi, int64_t offset, int64_t n,

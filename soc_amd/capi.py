@@ -198,6 +198,9 @@ def lib() -> C.CDLL:
         "soc_paged_append": (C.c_int, [P, P, P, P, I64, P, I64, P, I64, I32, P, I64, I32, I32, P, P]),
         "soc_paged_attention_decode": (C.c_int, [P, P, P, I64, I32, P, I64, I32, P, I32, I32, F32, P, I64, P]),
         "soc_logprobs": (C.c_int, [P, P, I32, I64, I32, I32, F32, P, P, P, P, I32, P, P]),
+        "soc_paged_fork": (C.c_int, [P, I32, P, P, P, I32, P, P, I32, I64, P, I32, P, P, P, P, P, P, P]),
+        "soc_paged_copy": (C.c_int, [P, P, I32, P, P, I32]),
+        "soc_paged_compact": (C.c_int, [P, I32, P, I32, P, P, I32, I64, P, P, I32, P, P, I32, P, P]),
         "soc_synth_normal_f16": (C.c_int, [U64, C.c_char_p, F32, I64, I64, P]),
         "soc_synth_uniform_f16": (C.c_int, [U64, C.c_char_p, F32, F32, I64, I64, P]),
         "soc_synth_tokens": (C.c_int, [U64, C.c_char_p, I32, I64, P]),
@@ -722,3 +725,32 @@ def logprobs(ctx: Context, logits: int, dtype: str, row_stride: int, rows: int, 
              top_ids: int | None, top_logprobs: int | None) -> None:
     check(lib().soc_logprobs(ctx.h, logits, DTYPES[dtype], row_stride, rows, vocab, temperature, tokens, logprobs,
                              ranks, entropy, top_n, top_ids, top_logprobs))
+
+
+# ---- rows that go on from other rows -----------------------------------------------------------------------------
+class PagedLayers:
+    """The caches of several layers, of one shape (what soc_paged_copy takes)."""
+
+    def __init__(self, caches: "list[PagedCache]"):
+        self.n = len(caches)
+        self.c = (PagedCacheC * max(1, self.n))(*[cache.c for cache in caches])
+
+
+def paged_fork(ctx: Context, n: int, parents: int, keep: int | None, old_lens: int, page_size: int, block_table: int,
+               new_table: int, max_pages: int, table_stride: int, free_ring: int, num_pages: int, cursors_in: int,
+               cursors_out: int, new_lens: int, next_lens: int | None, copies: int, copy_count: int,
+               status: int) -> None:
+    check(lib().soc_paged_fork(ctx.h, n, parents, keep, old_lens, page_size, block_table, new_table, max_pages,
+                               table_stride, free_ring, num_pages, cursors_in, cursors_out, new_lens, next_lens, copies,
+                               copy_count, status))
+
+
+def paged_copy(ctx: Context, layers: PagedLayers, moves: int, move_count: int | None, max_moves: int) -> None:
+    check(lib().soc_paged_copy(ctx.h, layers.c, layers.n, moves, move_count, max_moves))
+
+
+def paged_compact(ctx: Context, n: int, lens: int, page_size: int, block_table: int, new_table: int, max_pages: int,
+                  table_stride: int, free_ring: int, new_ring: int, num_pages: int, cursors: int, moves: int,
+                  max_moves: int, move_count: int, status: int) -> None:
+    check(lib().soc_paged_compact(ctx.h, n, lens, page_size, block_table, new_table, max_pages, table_stride, free_ring,
+                                  new_ring, num_pages, cursors, moves, max_moves, move_count, status))

@@ -50,6 +50,9 @@ struct soc_ctx {
   size_t serve_ws_bytes = 0;
   int* serve_counters = nullptr;
   size_t serve_counter_ints = 0;
+  // soc_paged_fork and soc_paged_compact: words kept for each page of a pool, grown on demand
+  uint32_t* page_words = nullptr;
+  int64_t page_words_pages = 0;
   // soc_forward with token ids in device memory: set by the staging kernel when an id lies outside [0, vocab)
   int* id_err = nullptr;
 };

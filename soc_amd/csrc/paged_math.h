@@ -85,4 +85,65 @@ SOC_HD PlanItem plan_item(int32_t before, int32_t after, int32_t max_pages, int 
   return p;
 }
 
+// What a row of a forked table asks for: the first `keep` positions of its parent, which holds `held` positions. `heir`: its
+// last page is partly filled by it and is the parent's own partly filled last page, which one such child may keep. A page
+// that the parent has filled counts as shared, whoever else holds it.
+struct ForkItem {
+  int32_t keep, pages;
+  bool partial, heir;
+  bool bad;  // a parent or a length out of range
+};
+SOC_HD ForkItem fork_item(int32_t parent, int32_t n, int32_t held, int32_t keep, int32_t max_pages, int page_shift) {
+  ForkItem f{0, 0, false, false, false};
+  if (parent == -1) return f;
+  if (parent < 0 || parent >= n || held < 0 || pages_of(held, page_shift) > max_pages || keep < 0 || keep > held) {
+    f.bad = true;
+    return f;
+  }
+  const int32_t inside = (1 << page_shift) - 1;
+  f.keep = keep;
+  f.pages = pages_of(keep, page_shift);
+  f.partial = (keep & inside) != 0;
+  f.heir = f.partial && (held & inside) != 0 && f.pages == pages_of(held, page_shift);
+  return f;
+}
+
+// A pool's pages as a bitmap, one bit a free page, with the free pages before each group of 2^group_shift words of 32:
+// counts[g], g <= the number of groups, the last of them all. Words hold no bit beyond the pool's pages.
+struct FreePages {
+  const uint32_t* words;
+  const int32_t* counts;
+  int group_shift, groups;
+};
+// Free pages below page p, 0 <= p <= the pool's pages.
+SOC_HD int32_t free_below(const FreePages& f, int32_t p) {
+  const int32_t w = p >> 5, g = w >> f.group_shift;
+  int32_t c = f.counts[g];
+  for (int32_t i = g << f.group_shift; i < w; ++i) c += __builtin_popcount(f.words[i]);
+  if ((p & 31) != 0) c += __builtin_popcount(f.words[w] & ((1u << (p & 31)) - 1u));
+  return c;
+}
+// The free page that `rank` free pages lie below, 0 <= rank < all of them.
+SOC_HD int32_t free_page(const FreePages& f, int32_t rank) {
+  int32_t lo = 0, hi = f.groups;  // counts[lo] <= rank < counts[hi]
+  while (hi - lo > 1) {
+    const int32_t mid = (lo + hi) >> 1;
+    if (f.counts[mid] <= rank) lo = mid;
+    else hi = mid;
+  }
+  int32_t left = rank - f.counts[lo], w = lo << f.group_shift;
+  const int32_t end = (lo + 1) << f.group_shift;
+  uint32_t word = f.words[w];
+  for (int32_t c = __builtin_popcount(word); left >= c && w + 1 < end; c = __builtin_popcount(word)) {
+    left -= c;
+    word = f.words[++w];
+  }
+  for (; left > 0; --left) word &= word - 1;
+  return (w << 5) + (word != 0 ? __builtin_ctz(word) : 0);
+}
+// Pages in use above page p.
+SOC_HD int32_t used_above(const FreePages& f, int32_t p, int32_t num_pages) {
+  return num_pages - 1 - p - (f.counts[f.groups] - free_below(f, p + 1));
+}
+
 }  // namespace soc

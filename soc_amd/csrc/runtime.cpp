@@ -1258,6 +1258,7 @@ int soc_ctx_destroy(soc_ctx* ctx) {
   (void)hipFree(ctx->op_counters);
   (void)hipFree(ctx->serve_ws);
   (void)hipFree(ctx->serve_counters);
+  (void)hipFree(ctx->page_words);
   (void)hipFree(ctx->id_err);
   delete ctx;
   return SOC_OK;

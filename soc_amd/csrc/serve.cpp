@@ -1,8 +1,8 @@
-// serve.cpp - what the paged serving entry points share on the host: the check of strided operands and the context's
-// workspace.
+// serve.cpp - what the paged serving entry points share on the host: the checks of strided operands and of a cache, and the
+// context's workspace.
 #include <string>
 
-#include "capi_internal.h"
+#include "paged_host.h"
 
 namespace soc {
 
@@ -45,6 +45,48 @@ int Operands::rows(const char* what, const void* p, int64_t rows, int64_t stride
   if (bytes > static_cast<uint64_t>(in->end - begin))
     return fail(SOC_ERR_INVALID, std::string(what) + " extends past the end of its device allocation");
   return SOC_OK;
+}
+
+int shift_of(int page_size) {
+  int s = 0;
+  while ((1 << s) < page_size) ++s;
+  return s;
+}
+
+int check_page_size(int32_t page_size) {
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
+    return fail(SOC_ERR_INVALID, "paged cache: page_size must be 16, 32, 64, 128 or 256");
+  return SOC_OK;
+}
+
+int check_cache_shape(const soc_paged_cache* c) {
+  if (c == nullptr) return fail(SOC_ERR_INVALID, "null paged cache");
+  SOC_TRY(check_page_size(c->page_size));
+  if (c->head_dim != 64 && c->head_dim != 128) return fail(SOC_ERR_INVALID, "paged cache: head_dim must be 64 or 128");
+  if (c->kv_heads <= 0 || c->kv_heads > 1024 || c->num_pages <= 0)
+    return fail(SOC_ERR_INVALID, "paged cache: need num_pages > 0 and 1 to 1024 kv_heads");
+  if (static_cast<int64_t>(c->num_pages) * c->page_size > INT32_MAX)
+    return fail(SOC_ERR_INVALID, "paged cache: num_pages * page_size must be below 2^31");
+  const int64_t page = static_cast<int64_t>(c->kv_heads) * c->page_size * c->head_dim;
+  if (c->page_stride != 0 && (c->page_stride < page || c->page_stride % 8 != 0))
+    return fail(SOC_ERR_INVALID, "paged cache: page_stride must be 0 or a multiple of 8 that holds a page");
+  if (reinterpret_cast<uintptr_t>(c->keys) % 16 != 0 || reinterpret_cast<uintptr_t>(c->values) % 16 != 0)
+    return fail(SOC_ERR_INVALID, "paged cache: keys and values must be 16-byte aligned");
+  return SOC_OK;
+}
+
+int64_t page_stride(const soc_paged_cache* c) {
+  return c->page_stride != 0 ? c->page_stride : static_cast<int64_t>(c->kv_heads) * c->page_size * c->head_dim;
+}
+
+int check_cache_memory(Operands& operands, const soc_paged_cache* c) {
+  const int64_t page = static_cast<int64_t>(c->kv_heads) * c->page_size * c->head_dim;
+  SOC_TRY(operands.rows("paged cache keys", c->keys, c->num_pages, page_stride(c), page, 2));
+  return operands.rows("paged cache values", c->values, c->num_pages, page_stride(c), page, 2);
+}
+
+int hip_status(hipError_t e, const char* what) {
+  return e == hipSuccess ? SOC_OK : fail(SOC_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
 
 int ensure_serve_ws(soc_ctx* ctx, size_t bytes, size_t ints) {
