@@ -436,6 +436,22 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
  *      otherwise write, all layers), then a step as above from the lengths that the fork gives, its attention by
  *      soc_paged_attention_shared. Rows that share pages end, or get shorter than what they share, by a fork and not by a
  *      plan (which gives back each row's pages, whoever else names them). What holds for the calls above holds here. ---- */
+/* The best continuations of `groups` requests with `beams` (1 to 64) beams each, at most 2^20 rows of logits (row g * beams +
+ * b; `vocab` logits of SOC_DTYPE_F32 or _F16, at most 2^20, row_stride elements apart): the score of token v behind row r is
+ * scores[r] + the log probability of v under softmax(row r / temperature) (temperature <= 0 taken as 1; at most 2^100). The
+ * order of a request's continuations is by score, greater first; equal scores by lowest row, then as in soc_logprobs (by
+ * logit, then lowest id). Scores are formed and compared in 64 bits and rounded to fp32 once.
+ *   top_rows, top_tokens, top_scores [groups][top_n] (0 <= top_n <= 64; NULL at 0): the first top_n.
+ *   next_rows, next_tokens, next_scores [groups * beams] (all or none NULL): each request's first `beams` whose token is none
+ *     of stop_tokens [num_stops] (host memory; at most 8, and beams * (1 + num_stops) at most 64): its next beams, of which
+ *     next_rows are the parents that soc_paged_fork takes. next_scores may be scores.
+ * Where there are fewer, row and token are -1 and the score is -inf. Tokens of logit -inf, rows whose score is no finite
+ * number (-inf: a beam that is none), and rows that hold a NaN or +inf offer nothing. A request's results do not depend on
+ * the other requests, nor on the rows' alignment. */
+int soc_beam_select(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_stride, int32_t groups, int32_t beams,
+                    int32_t vocab, float temperature, const float* scores, const int32_t* stop_tokens, int32_t num_stops,
+                    int32_t top_n, int32_t* top_rows, int32_t* top_tokens, float* top_scores, int32_t* next_rows,
+                    int32_t* next_tokens, float* next_scores);
 /* The table after row i has gone on from row parents[i] (-1: it ends) with its first keep[i] positions (keep NULL: all that
  * old_lens[parents[i]] says); 1 <= n <= 4096 rows, and they are all that hold pages: new_table row i names its parent's
  * pages, but where keep[i] ends inside a page, that page is new, taken from the ring's head in order of the rows, and to be

@@ -198,6 +198,7 @@ def lib() -> C.CDLL:
         "soc_paged_append": (C.c_int, [P, P, P, P, I64, P, I64, P, I64, I32, P, I64, I32, I32, P, P]),
         "soc_paged_attention_decode": (C.c_int, [P, P, P, I64, I32, P, I64, I32, P, I32, I32, F32, P, I64, P]),
         "soc_logprobs": (C.c_int, [P, P, I32, I64, I32, I32, F32, P, P, P, P, I32, P, P]),
+        "soc_beam_select": (C.c_int, [P, P, I32, I64, I32, I32, I32, F32, P, P, I32, I32, P, P, P, P, P, P]),
         "soc_paged_fork": (C.c_int, [P, I32, P, P, P, I32, P, P, I32, I64, P, I32, P, P, P, P, P, P, P]),
         "soc_paged_copy": (C.c_int, [P, P, I32, P, P, I32]),
         "soc_paged_compact": (C.c_int, [P, I32, P, I32, P, P, I32, I64, P, P, I32, P, P, I32, P, P]),
@@ -728,6 +729,17 @@ def logprobs(ctx: Context, logits: int, dtype: str, row_stride: int, rows: int, 
 
 
 # ---- rows that go on from other rows -----------------------------------------------------------------------------
+def beam_select(ctx: Context, logits: int, dtype: str, row_stride: int, groups: int, beams: int, vocab: int,
+                temperature: float, scores: int, stop_tokens, top_n: int, top_rows: int | None, top_tokens: int | None,
+                top_scores: int | None, next_rows: int | None, next_tokens: int | None,
+                next_scores: int | None) -> None:
+    """soc_beam_select; stop_tokens: a sequence of token ids."""
+    stops = (C.c_int32 * max(1, len(stop_tokens)))(*stop_tokens)
+    check(lib().soc_beam_select(ctx.h, logits, DTYPES[dtype], row_stride, groups, beams, vocab, temperature, scores,
+                                stops, len(stop_tokens), top_n, top_rows, top_tokens, top_scores, next_rows,
+                                next_tokens, next_scores))
+
+
 class PagedLayers:
     """The caches of several layers, of one shape (what soc_paged_copy takes)."""
 

@@ -13,12 +13,10 @@
 #include <string>
 
 #include "capi_internal.h"
-#include "device_common.h"
+#include "top_keys.h"
 
 namespace soc {
 namespace {
-
-constexpr int kMaxTop = 64;
 
 struct LogprobArgs {
   const void* logits;
@@ -40,43 +38,14 @@ struct LogprobArgs {
   int* arrived;          // [rows], zero between launches
 };
 
-// Order of logits as unsigned words: NaNs first, then by value, both zeros alike; never 0 nor all ones. A 16-bit logit's
-// order is in the upper half.
-constexpr uint32_t kOrderNan = 0xffff0000u;  // above +inf's 0xff800000 (16 bits: 0xfc000000)
-template <typename T>
-__device__ __forceinline__ uint32_t order_of(float x) {
-  if (x != x) return kOrderNan;
-  uint32_t b = __float_as_uint(x + 0.0f);
-  if constexpr (sizeof(T) == 2) b = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<f16>(x + 0.0f))) << 16;
-  const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return sizeof(T) == 2 ? o & 0xffff0000u : o;
-}
-template <typename T>
-__device__ __forceinline__ float value_of(uint32_t o) {
-  if (o == kOrderNan) return __builtin_nanf("");
-  const uint32_t b = o & 0x80000000u ? o & 0x7fffffffu : ~o;
-  if constexpr (sizeof(T) == 2) return static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(b >> 16)));
-  return __uint_as_float(b);
-}
-// Order of tokens: by logit, then by lowest id. Distinct for every token of a row; 0 is below all of them.
-constexpr int kMaxVocab = 1 << 20;
-__device__ __forceinline__ uint32_t low_of(int id) { return static_cast<uint32_t>(kMaxVocab - id); }  // 1 .. 2^20
-template <typename T>
-__device__ __forceinline__ uint64_t key_of(float x, int id) {
-  return static_cast<uint64_t>(order_of<T>(x)) << 32 | low_of(id);
-}
-
 // One block per chunk of a row: 256 threads with E logits each in registers, read once in 16-byte loads, all requested
 // before the first is used. The chunk's maximum comes first, so that every exponential is taken once; each thread counts
-// its tokens before the given one, and one sum over the block follows. Of the top n, each thread's largest token stands
-// for its E: the n-th largest of those 256 keys is a threshold that at most n threads reach, so at most n E tokens (64 of
-// normal data) are candidates, and those rank each other. No step depends on how many values are equal. The last block of
-// a row to finish joins its chunks, in chunk order.
+// its tokens before the given one, and one sum over the block follows; then the chunk's top n (block_first). The last block
+// of a row to finish joins its chunks, in chunk order.
 // 777 rows of 151936 fp32 logits with top 8 take 96 us (4.9 TB/s; 87 us without alternatives, 5.4 TB/s). The same in fp16
 // takes 87 us, so there the instructions a logit count, not memory. One row takes 10.7 us with top 20 and 5.3 without:
 // the chain of reading, reducing, selecting, handing over and joining. At 32 fp32 logits a thread, 64 registers (8 waves
 // a SIMD) are worth 5 % on many rows; in 16 bits they would spill.
-constexpr int kThreads = 256;
 // Keys in LDS: the candidates of a chunk (top_n threads of E tokens); then the top_n of every chunk that one block joins,
 // and those of them at the threshold.
 __host__ __device__ constexpr int key_room(int top_n, int each, int chunks) {
@@ -88,97 +57,16 @@ struct Part {  // of a chunk: largest logit, sum of 2^d, sum of d 2^d (d: base-2
   int above;
 };
 
-// How many of the wave's words, K a lane, are not below x.
-template <int K>
-__device__ __forceinline__ int reaching(const uint32_t (&w)[K], uint32_t x) {
-  int c = 0;
-#pragma unroll
-  for (int j = 0; j < K; ++j) c += __popcll(__ballot(w[j] >= x));
-  return c;
-}
-// Largest and smallest word of the wave (DPP within rows of 16, then the four rows).
-template <typename F>
-__device__ __forceinline__ uint32_t wave_fold(uint32_t v, F f) {
-  v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xB1, 0xF, 0xF, true)));
-  v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4E, 0xF, 0xF, true)));
-  v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x141, 0xF, 0xF, true)));
-  v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x140, 0xF, 0xF, true)));
-  const auto row = [&](int lane) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane)); };
-  return __builtin_amdgcn_readfirstlane(f(f(row(0), row(16)), f(row(32), row(48))));
-}
-// The largest x with bits from `low` up that at least n <= 64 K of the wave's words reach (0 where fewer are above 0), by
-// bisection with ballots from the first bit in which the words differ. Ends as soon as exactly n reach it: *exact. That
-// is after about ten bits of the orders of ordinary logits.
-template <int K>
-__device__ __forceinline__ uint32_t nth_word(const uint32_t (&w)[K], int n, int low, bool* exact) {
-  uint32_t most = w[0], least = w[0];
-#pragma unroll
-  for (int j = 1; j < K; ++j) {
-    most = max(most, w[j]);
-    least = min(least, w[j]);
-  }
-  most = wave_fold(most, [](uint32_t x, uint32_t y) { return max(x, y); });
-  least = wave_fold(least, [](uint32_t x, uint32_t y) { return min(x, y); });
-  const uint32_t differ = most ^ least;
-  const int top = differ == 0 ? -1 : 31 - __builtin_clz(differ);
-  // the bits that all words share: 64 bits, so that the shift by 32 is one
-  uint32_t t = most & static_cast<uint32_t>(~0ull << (top + 1));
-  *exact = false;
-  for (int bit = top; bit >= low; --bit) {
-    const uint32_t x = t | 1u << bit;
-    const int c = reaching(w, x);
-    if (c >= n) t = x;
-    if (c == n) {
-      *exact = true;
-      break;
-    }
-  }
-  return t;
-}
-// The n-th largest of `count` <= 64 K keys (distinct, or 0 for none), by the calling wave: at least 1; where there are
-// fewer than n keys, none is below it. First the orders, then the ids among equal orders.
-template <typename T, int K, typename Key>
-__device__ __forceinline__ uint64_t nth_largest(Key key, int count, int n) {
-  constexpr int kLow = sizeof(T) == 2 ? 16 : 0;
-  const int lane = threadIdx.x & (kWave - 1);
-  uint32_t w[K];
-#pragma unroll
-  for (int j = 0; j < K; ++j)
-    w[j] = j * kWave + lane < count ? static_cast<uint32_t>(key(j * kWave + lane) >> 32) : 0;
-  bool exact;
-  const uint32_t t = nth_word(w, n, kLow, &exact);
-  if (exact) return static_cast<uint64_t>(t) << 32;
-  if (t == 0) return 1;
-  const int ties = n - reaching(w, t + 1);  // wanted of those of order t
-#pragma unroll
-  for (int j = 0; j < K; ++j) w[j] = w[j] == t ? static_cast<uint32_t>(key(j * kWave + lane)) : 0;
-  return static_cast<uint64_t>(t) << 32 | nth_word(w, ties, 0, &exact);
-}
-
-// The n largest of `count` distinct keys in LDS, in order, to `first`, by all threads: each key counts the larger ones.
-__device__ __forceinline__ void rank_first(const uint64_t* keys, int count, int n, uint64_t* first) {
-  for (int i = threadIdx.x; i < count; i += kThreads) {
-    const uint64_t key = keys[i];
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < count; ++j) rank += keys[j] > key;
-    if (rank < n) first[rank] = key;
-  }
-}
-
 template <typename T, int E>
 __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k_logprobs(LogprobArgs a) {
   constexpr int VW = 16 / sizeof(T), NV = E / VW, C = kThreads * E;
-  constexpr int kLow = sizeof(T) == 2 ? 16 : 0;  // lowest bit of an order
   typedef T Vec __attribute__((ext_vector_type(VW)));
   extern __shared__ uint64_t keys[];  // key_room(top_n, E, chunks)
-  __shared__ uint64_t group[kThreads];
+  __shared__ BlockTop top;
   __shared__ uint64_t first[kMaxTop];
   __shared__ float red[3][4];
   __shared__ int count[4];
-  __shared__ uint64_t threshold;
-  __shared__ int giver[kMaxTop];
-  __shared__ int found, givers, last, tied;
+  __shared__ int last;
 
   const int64_t r = blockIdx.x / a.chunks;
   const int c = blockIdx.x % a.chunks;
@@ -226,7 +114,7 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   for (int e = 1; e < E; ++e) best = fmaxf(best, v[e]);
   float m = wave_max(best);
   if (lane == 0) red[0][wid] = m;
-  if (tid == 0) found = givers = 0;
+  if (tid == 0) top.found = top.givers = 0;
   __syncthreads();
   m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   // -inf alone sums to 0; NaN, or +inf less itself, makes the sums NaN
@@ -284,84 +172,7 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
 
   const int n = a.top_n;
   if (n > 0) {
-    // the order of the thread's largest; 0 where it has no logit (the lowest of its ids is place(0), or 0). Where the sum
-    // is NaN, a NaN may hide from `best`
-    uint32_t order = place(0) < a.vocab ? order_of<T>(best) : 0;
-    if (s != s) {
-      order = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (place(e) >= 0 && place(e) < a.vocab) order = max(order, order_of<T>(v[e]));
-    }
-    group[tid] = static_cast<uint64_t>(order) << 32;
-    __syncthreads();
-    uint32_t w[kThreads / kWave];  // wave 0
-    if (wid == 0) {
-#pragma unroll
-      for (int j = 0; j < kThreads / kWave; ++j) w[j] = static_cast<uint32_t>(group[j * kWave + lane] >> 32);
-      bool exact;
-      const uint32_t o = nth_word(w, n, kLow, &exact);
-      if (lane == 0) {
-        threshold = static_cast<uint64_t>(o) << 32;
-        tied = !exact && o != 0;
-      }
-    }
-    __syncthreads();
-    if (tied) {  // threads whose largest are equal at the threshold: those of the lowest ids
-      const uint32_t o = static_cast<uint32_t>(threshold >> 32);
-      if (order == o) {
-        const float ov = value_of<T>(o);
-        int id = 0;
-#pragma unroll
-        for (int e = E - 1; e >= 0; --e)
-          if ((v[e] == ov || (v[e] != v[e] && ov != ov)) && place(e) >= 0 && place(e) < a.vocab) id = place(e);
-        group[tid] |= low_of(id);
-      }
-      __syncthreads();
-      if (wid == 0) {
-        const int ties = n - reaching(w, o + 1);
-#pragma unroll
-        for (int j = 0; j < kThreads / kWave; ++j)
-          w[j] = w[j] == o ? static_cast<uint32_t>(group[j * kWave + lane]) : 0;
-        bool exact;
-        const uint32_t low = nth_word(w, ties, 0, &exact);
-        if (lane == 0) threshold |= low;
-      }
-    }
-    if (tid < n) first[tid] = 0;
-    __syncthreads();
-    const uint64_t t = max(threshold, uint64_t{1});
-    const float tv = value_of<T>(static_cast<uint32_t>(t >> 32));
-    // the logits of the threads that reach it, at most n, are handed to all threads: E registers tested in place would be
-    // E copies of what follows, mostly skipped (one row top 20 11.6 us for 10.7, 777 fp16 rows 91 for 87)
-    float* handed = reinterpret_cast<float*>(keys);
-    if (group[tid] >= t) {
-      const int at = atomicAdd(&givers, 1);
-      giver[at] = tid;
-#pragma unroll
-      for (int e = 0; e < E; ++e) handed[at * E + e] = v[e];
-    }
-    __syncthreads();
-    const int all = __builtin_amdgcn_readfirstlane(givers * E);
-    float y[kMaxTop * E / kThreads];
-#pragma unroll
-    for (int k = 0; k < kMaxTop * E / kThreads; ++k) {
-      if (k * kThreads >= all) break;
-      y[k] = handed[min(k * kThreads + tid, all - 1)];
-    }
-    __syncthreads();  // the keys take the logits' place
-#pragma unroll
-    for (int k = 0; k < kMaxTop * E / kThreads; ++k) {
-      if (k * kThreads >= all) break;
-      const int i = k * kThreads + tid;
-      if (i < all && !(y[k] < tv)) {
-        const int id = place_of(giver[i / E], i % E);
-        const uint64_t key = key_of<T>(y[k], id);
-        if (id >= 0 && id < a.vocab && key >= t) keys[atomicAdd(&found, 1)] = key;
-      }
-    }
-    __syncthreads();
-    rank_first(keys, found, n, first);
+    block_first<T, E>(v, best, s != s, place, place_of, a.vocab, n, keys, top, first);
     __syncthreads();
   }
 
@@ -411,19 +222,19 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
       const int all = a.chunks * n, few = min(n, (n - 1) / a.chunks + 2);  // at most 64 + 2 * 65 words
       uint64_t* left = keys + all;
       __syncthreads();
-      if (tid == 0) found = 0;
+      if (tid == 0) top.found = 0;
       if (wid == 0) {
         const auto key = [&](int i) { return keys[i / few * n + i % few]; };
         const uint64_t t = a.chunks * few <= kWave ? nth_largest<T, 1>(key, a.chunks * few, n)
                                                    : nth_largest<T, 4>(key, a.chunks * few, n);
-        if (lane == 0) threshold = t;
+        if (lane == 0) top.threshold = t;
       }
       __syncthreads();
-      const uint64_t t = threshold;
+      const uint64_t t = top.threshold;
       for (int i = tid; i < all; i += kThreads)
-        if (keys[i] >= t) left[atomicAdd(&found, 1)] = keys[i];
+        if (keys[i] >= t) left[atomicAdd(&top.found, 1)] = keys[i];
       __syncthreads();
-      rank_first(left, found, n, first);
+      rank_first(left, top.found, n, first);
       __syncthreads();
     }
   }

@@ -73,3 +73,20 @@ def test_copy_refusals(second, layers, moves, text):
 
 def test_copy_needs_caches():
     refused(lib().soc_paged_copy(None, None, 2, SOME, SOME, 4), "null paged cache")
+
+
+@pytest.mark.parametrize("kw,text", [
+    ({"dtype": 2}, "dtype"), ({"groups": 0}, "groups"), ({"beams": 0}, "64 beams"), ({"beams": 65}, "64 beams"),
+    ({"groups": 1 << 19}, "2^20 rows"), ({"vocab": 0}, "vocabulary"), ({"vocab": (1 << 20) + 1}, "vocabulary"),
+    ({"temperature": float("nan")}, "temperature"), ({"temperature": float("inf")}, "temperature"),
+    ({"temperature": 2e30}, "temperature"), ({"temperature": 1e-39}, "temperature"), ({"stops": -1}, "stop tokens"),
+    ({"stops": 9}, "stop tokens"), ({"stop_p": None}, "stop tokens"), ({"top": -1}, "top_n"), ({"top": 65}, "top_n"),
+    ({"beams": 22, "stops": 2}, "at most 64"), ({"next": None, "top": 0}, "nothing"), ({}, "null context"),
+    ({"beams": 22, "stops": 2, "next": None}, "null context"), ({"top": 0}, "null context"),
+])
+def test_beam_refusals(kw, text):
+    a = dict(dtype=0, groups=2, beams=4, vocab=100, temperature=1.0, stops=1, stop_p=(C.c_int32 * 9)(), top=8, next=SOME)
+    a.update(kw)
+    refused(lib().soc_beam_select(None, SOME, a["dtype"], a["vocab"], a["groups"], a["beams"], a["vocab"], a["temperature"],
+                                  SOME, a["stop_p"], a["stops"], a["top"], SOME, SOME, SOME, a["next"], a["next"],
+                                  a["next"]), text)
