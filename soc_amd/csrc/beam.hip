@@ -77,6 +77,100 @@ __device__ __forceinline__ double score_value(uint64_t o) {
   return __builtin_bit_cast(double, o >> 63 ? o & ~(uint64_t{1} << 63) : ~o);
 }
 
+// The n first tokens of a block's chunk, in order, to `first` (0 where it has fewer; a barrier before it is read), by all
+// threads. A thread holds E logits v, logit e of id place(e) (of another thread: place_of(thread, e)), its largest `best`;
+// ids outside [0, vocab) are no tokens and their logits -inf. keys: n * E words of LDS. Each thread's largest token stands
+// for its E: the n-th largest of those keys is a threshold that at most n threads reach, so at most n E tokens (64 of
+// normal data) are candidates, and those rank each other. No step depends on how many values are equal. nans: whether a NaN
+// may be among the logits. The rest is LDS; found and givers are 0 before the call, with a barrier since. (soc_logprobs has
+// these steps in its kernel: calling this takes it 0.3 us of 11 for one row.)
+template <typename T, int E, typename Place, typename PlaceOf>
+__device__ __forceinline__ void block_first(const float (&v)[E], float best, bool nans, Place place, PlaceOf place_of,
+                                            int vocab, int n, uint64_t* keys, uint64_t* first,
+                                            uint64_t (&group)[kThreads], uint64_t& threshold, int (&giver)[kMaxTop],
+                                            int& found, int& givers, int& tied) {
+  constexpr int kLow = sizeof(T) == 2 ? 16 : 0;  // lowest bit of an order
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
+  // the order of the thread's largest; 0 where it has no logit (the lowest of its ids is place(0), or 0). Where the sum
+  // is NaN, a NaN may hide from `best`
+  uint32_t order = place(0) < vocab ? order_of<T>(best) : 0;
+  if (nans) {
+    order = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (place(e) >= 0 && place(e) < vocab) order = max(order, order_of<T>(v[e]));
+  }
+  group[tid] = static_cast<uint64_t>(order) << 32;
+  __syncthreads();
+  uint32_t w[kThreads / kWave];  // wave 0
+  if (wid == 0) {
+#pragma unroll
+    for (int j = 0; j < kThreads / kWave; ++j) w[j] = static_cast<uint32_t>(group[j * kWave + lane] >> 32);
+    bool exact;
+    const uint32_t o = nth_word(w, n, kLow, &exact);
+    if (lane == 0) {
+      threshold = static_cast<uint64_t>(o) << 32;
+      tied = !exact && o != 0;
+    }
+  }
+  __syncthreads();
+  if (tied) {  // threads whose largest are equal at the threshold: those of the lowest ids
+    const uint32_t o = static_cast<uint32_t>(threshold >> 32);
+    if (order == o) {
+      const float ov = value_of<T>(o);
+      int id = 0;
+#pragma unroll
+      for (int e = E - 1; e >= 0; --e)
+        if ((v[e] == ov || (v[e] != v[e] && ov != ov)) && place(e) >= 0 && place(e) < vocab) id = place(e);
+      group[tid] |= low_of(id);
+    }
+    __syncthreads();
+    if (wid == 0) {
+      const int ties = n - reaching(w, o + 1);
+#pragma unroll
+      for (int j = 0; j < kThreads / kWave; ++j)
+        w[j] = w[j] == o ? static_cast<uint32_t>(group[j * kWave + lane]) : 0;
+      bool exact;
+      const uint32_t low = nth_word(w, ties, 0, &exact);
+      if (lane == 0) threshold |= low;
+    }
+  }
+  if (tid < n) first[tid] = 0;
+  __syncthreads();
+  const uint64_t t = max(threshold, uint64_t{1});
+  const float tv = value_of<T>(static_cast<uint32_t>(t >> 32));
+  // the logits of the threads that reach it, at most n, are handed to all threads: E registers tested in place would be
+  // E copies of what follows, mostly skipped (one row top 20 11.6 us for 10.7, 777 fp16 rows 91 for 87)
+  float* handed = reinterpret_cast<float*>(keys);
+  if (group[tid] >= t) {
+    const int at = atomicAdd(&givers, 1);
+    giver[at] = tid;
+#pragma unroll
+    for (int e = 0; e < E; ++e) handed[at * E + e] = v[e];
+  }
+  __syncthreads();
+  const int all = __builtin_amdgcn_readfirstlane(givers * E);
+  float y[kMaxTop * E / kThreads];
+#pragma unroll
+  for (int k = 0; k < kMaxTop * E / kThreads; ++k) {
+    if (k * kThreads >= all) break;
+    y[k] = handed[min(k * kThreads + tid, all - 1)];
+  }
+  __syncthreads();  // the keys take the logits' place
+#pragma unroll
+  for (int k = 0; k < kMaxTop * E / kThreads; ++k) {
+    if (k * kThreads >= all) break;
+    const int i = k * kThreads + tid;
+    if (i < all && !(y[k] < tv)) {
+      const int id = place_of(giver[i / E], i % E);
+      const uint64_t key = key_of<T>(y[k], id);
+      if (id >= 0 && id < vocab && key >= t) keys[atomicAdd(&found, 1)] = key;
+    }
+  }
+  __syncthreads();
+  rank_first(keys, found, n, first);
+}
+
 // LDS beside the static: a chunk's candidates, or the first n of every chunk and those of them at the threshold; then the
 // scores of every beam's first n, and which of them are at the threshold.
 __host__ __device__ constexpr size_t beam_room(int n, int each, int chunks, int beams) {
@@ -91,10 +185,12 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   constexpr int VW = 16 / sizeof(T), NV = E / VW, C = kThreads * E;
   typedef T Vec __attribute__((ext_vector_type(VW), aligned(sizeof(T))));
   extern __shared__ uint64_t keys[];  // beam_room
-  __shared__ BlockTop top;
+  __shared__ uint64_t group[kThreads];
   __shared__ uint64_t first[kMaxTop];
   __shared__ float red[2][4];
-  __shared__ int flag;
+  __shared__ uint64_t threshold;
+  __shared__ int giver[kMaxTop];
+  __shared__ int found, givers, flag, tied;
 
   const int64_t r = blockIdx.x / a.chunks;  // of the launch
   const int c = blockIdx.x % a.chunks, n = a.n;
@@ -129,7 +225,7 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   for (int e = 1; e < E; ++e) best = fmaxf(best, v[e]);
   float m = wave_max(best);
   if (lane == 0) red[0][wid] = m;
-  if (tid == 0) top.found = top.givers = 0;
+  if (tid == 0) found = givers = 0;
   __syncthreads();
   m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   // -inf alone sums to 0; NaN, or +inf less itself, makes the sum NaN
@@ -143,7 +239,8 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   part = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
   block_first<T, E>(
       v, best, part != part, [&](int e) { return base + (e / VW) * kThreads * VW + e % VW; },
-      [&](int thread, int e) { return lo + (thread + e / VW * kThreads) * VW + e % VW; }, a.vocab, n, keys, top, first);
+      [&](int thread, int e) { return lo + (thread + e / VW * kThreads) * VW + e % VW; }, a.vocab, n, keys, first, group,
+      threshold, giver, found, givers, tied);
   __syncthreads();
 
   double s = part;
@@ -163,21 +260,21 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
     // the first few of each chunk give a threshold that at least n of all keys reach, and seldom many more
     const int all = a.chunks * n, few = min(n, (n - 1) / a.chunks + 2);
     uint64_t* left = keys + all;
-    if (tid == 0) top.found = 0;
+    if (tid == 0) found = 0;
     __syncthreads();
     if (wid == 0) {
       const auto key = [&](int i) { return keys[i / few * n + i % few]; };
       const uint64_t t = a.chunks * few <= kWave ? nth_largest<T, 1>(key, a.chunks * few, n)
                                                  : nth_largest<T, 4>(key, a.chunks * few, n);
-      if (lane == 0) top.threshold = t;
+      if (lane == 0) threshold = t;
     }
     if (tid < n) first[tid] = 0;
     __syncthreads();
-    const uint64_t t = top.threshold;
+    const uint64_t t = threshold;
     for (int i = tid; i < all; i += kThreads)
-      if (keys[i] >= t) left[atomicAdd(&top.found, 1)] = keys[i];
+      if (keys[i] >= t) left[atomicAdd(&found, 1)] = keys[i];
     __syncthreads();
-    rank_first(left, top.found, n, first);
+    rank_first(left, found, n, first);
     __syncthreads();
   }
 
@@ -195,7 +292,7 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   const uint64_t* row_tops = a.row_tops + static_cast<int64_t>(row0) * n;
   uint64_t* scores = keys;
   int* left = reinterpret_cast<int*>(keys + all);
-  if (tid == 0) top.found = 0;
+  if (tid == 0) found = 0;
   for (int i = tid; i < all; i += kThreads) {
     const int b = i / n;
     const uint64_t key = ld_agent(row_tops + i);
@@ -207,7 +304,7 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
     // no token; a masked one; a beam that is none or whose row offers nothing
     scores[i] = key == 0 || !(score > -INFINITY) || !(score < INFINITY) ? 0 : score_order(score);
   }
-  if (tid < n) top.group[tid] = ~uint64_t{0};
+  if (tid < n) group[tid] = ~uint64_t{0};
   __syncthreads();
   // candidates: all, or where they are many those at a threshold that at least n reach
   uint32_t t = 1;
@@ -222,48 +319,48 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
       }
       bool exact;
       const uint32_t o = nth_word(w, n, 0, &exact);
-      if (lane == 0) top.threshold = max(o, 1u);
+      if (lane == 0) threshold = max(o, 1u);
     }
     __syncthreads();
-    t = static_cast<uint32_t>(top.threshold);
+    t = static_cast<uint32_t>(threshold);
   }
   for (int i = tid; i < all; i += kThreads)
-    if (scores[i] >> 32 >= t) left[atomicAdd(&top.found, 1)] = i;
+    if (scores[i] >> 32 >= t) left[atomicAdd(&found, 1)] = i;
   __syncthreads();
-  const int found = top.found;
-  for (int k = tid; k < found; k += kThreads) {
+  const int many = found;
+  for (int k = tid; k < many; k += kThreads) {
     const int i = left[k];
     const uint64_t score = scores[i];
     int rank = 0;
-    for (int u = 0; u < found; ++u) {
+    for (int u = 0; u < many; ++u) {
       const int j = left[u];
       const uint64_t other = scores[j];
       rank += other > score || (other == score && j < i);
     }
-    if (rank < n) top.group[rank] = i;
+    if (rank < n) group[rank] = i;
   }
   __syncthreads();
   if (wid != 0) return;
   int row = -1, token = -1;
   float score = -INFINITY;
-  if (lane < n && top.group[lane] != ~uint64_t{0}) {
-    const int i = static_cast<int>(top.group[lane]);
+  if (lane < n && group[lane] != ~uint64_t{0}) {
+    const int i = static_cast<int>(group[lane]);
     row = a.first_row + row0 + i / n;
     token = kMaxVocab - static_cast<int32_t>(static_cast<uint32_t>(ld_agent(row_tops + i)));
     score = static_cast<float>(score_value(scores[i]));
   }
-  const int64_t group = a.first_row / a.beams + g;
+  const int64_t request = a.first_row / a.beams + g;
   if (lane < a.top_n) {
-    a.top_rows[group * a.top_n + lane] = row;
-    a.top_tokens[group * a.top_n + lane] = token;
-    a.top_scores[group * a.top_n + lane] = score;
+    a.top_rows[request * a.top_n + lane] = row;
+    a.top_tokens[request * a.top_n + lane] = token;
+    a.top_scores[request * a.top_n + lane] = score;
   }
   if (a.next_rows == nullptr) return;
   bool goes_on = row >= 0;
   for (int k = 0; k < a.num_stops; ++k) goes_on &= token != a.stops[k];
   const uint64_t on = __ballot(goes_on);
   const int place = __popcll(on & ((uint64_t{1} << lane) - 1)), some = __popcll(on);
-  const int64_t out = group * a.beams;
+  const int64_t out = request * a.beams;
   if (goes_on && place < a.beams) {
     a.next_rows[out + place] = row;
     a.next_tokens[out + place] = token;

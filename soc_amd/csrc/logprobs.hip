@@ -40,8 +40,10 @@ struct LogprobArgs {
 
 // One block per chunk of a row: 256 threads with E logits each in registers, read once in 16-byte loads, all requested
 // before the first is used. The chunk's maximum comes first, so that every exponential is taken once; each thread counts
-// its tokens before the given one, and one sum over the block follows; then the chunk's top n (block_first). The last block
-// of a row to finish joins its chunks, in chunk order.
+// its tokens before the given one, and one sum over the block follows. Of the top n, each thread's largest token stands
+// for its E: the n-th largest of those 256 keys is a threshold that at most n threads reach, so at most n E tokens (64 of
+// normal data) are candidates, and those rank each other. No step depends on how many values are equal. The last block of
+// a row to finish joins its chunks, in chunk order.
 // 777 rows of 151936 fp32 logits with top 8 take 96 us (4.9 TB/s; 87 us without alternatives, 5.4 TB/s). The same in fp16
 // takes 87 us, so there the instructions a logit count, not memory. One row takes 10.7 us with top 20 and 5.3 without:
 // the chain of reading, reducing, selecting, handing over and joining. At 32 fp32 logits a thread, 64 registers (8 waves
@@ -60,13 +62,16 @@ struct Part {  // of a chunk: largest logit, sum of 2^d, sum of d 2^d (d: base-2
 template <typename T, int E>
 __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k_logprobs(LogprobArgs a) {
   constexpr int VW = 16 / sizeof(T), NV = E / VW, C = kThreads * E;
+  constexpr int kLow = sizeof(T) == 2 ? 16 : 0;  // lowest bit of an order
   typedef T Vec __attribute__((ext_vector_type(VW)));
   extern __shared__ uint64_t keys[];  // key_room(top_n, E, chunks)
-  __shared__ BlockTop top;
+  __shared__ uint64_t group[kThreads];
   __shared__ uint64_t first[kMaxTop];
   __shared__ float red[3][4];
   __shared__ int count[4];
-  __shared__ int last;
+  __shared__ uint64_t threshold;
+  __shared__ int giver[kMaxTop];
+  __shared__ int found, givers, last, tied;
 
   const int64_t r = blockIdx.x / a.chunks;
   const int c = blockIdx.x % a.chunks;
@@ -114,7 +119,7 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   for (int e = 1; e < E; ++e) best = fmaxf(best, v[e]);
   float m = wave_max(best);
   if (lane == 0) red[0][wid] = m;
-  if (tid == 0) top.found = top.givers = 0;
+  if (tid == 0) found = givers = 0;
   __syncthreads();
   m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   // -inf alone sums to 0; NaN, or +inf less itself, makes the sums NaN
@@ -172,7 +177,84 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
 
   const int n = a.top_n;
   if (n > 0) {
-    block_first<T, E>(v, best, s != s, place, place_of, a.vocab, n, keys, top, first);
+    // the order of the thread's largest; 0 where it has no logit (the lowest of its ids is place(0), or 0). Where the sum
+    // is NaN, a NaN may hide from `best`
+    uint32_t order = place(0) < a.vocab ? order_of<T>(best) : 0;
+    if (s != s) {
+      order = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (place(e) >= 0 && place(e) < a.vocab) order = max(order, order_of<T>(v[e]));
+    }
+    group[tid] = static_cast<uint64_t>(order) << 32;
+    __syncthreads();
+    uint32_t w[kThreads / kWave];  // wave 0
+    if (wid == 0) {
+#pragma unroll
+      for (int j = 0; j < kThreads / kWave; ++j) w[j] = static_cast<uint32_t>(group[j * kWave + lane] >> 32);
+      bool exact;
+      const uint32_t o = nth_word(w, n, kLow, &exact);
+      if (lane == 0) {
+        threshold = static_cast<uint64_t>(o) << 32;
+        tied = !exact && o != 0;
+      }
+    }
+    __syncthreads();
+    if (tied) {  // threads whose largest are equal at the threshold: those of the lowest ids
+      const uint32_t o = static_cast<uint32_t>(threshold >> 32);
+      if (order == o) {
+        const float ov = value_of<T>(o);
+        int id = 0;
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e)
+          if ((v[e] == ov || (v[e] != v[e] && ov != ov)) && place(e) >= 0 && place(e) < a.vocab) id = place(e);
+        group[tid] |= low_of(id);
+      }
+      __syncthreads();
+      if (wid == 0) {
+        const int ties = n - reaching(w, o + 1);
+#pragma unroll
+        for (int j = 0; j < kThreads / kWave; ++j)
+          w[j] = w[j] == o ? static_cast<uint32_t>(group[j * kWave + lane]) : 0;
+        bool exact;
+        const uint32_t low = nth_word(w, ties, 0, &exact);
+        if (lane == 0) threshold |= low;
+      }
+    }
+    if (tid < n) first[tid] = 0;
+    __syncthreads();
+    const uint64_t t = max(threshold, uint64_t{1});
+    const float tv = value_of<T>(static_cast<uint32_t>(t >> 32));
+    // the logits of the threads that reach it, at most n, are handed to all threads: E registers tested in place would be
+    // E copies of what follows, mostly skipped (one row top 20 11.6 us for 10.7, 777 fp16 rows 91 for 87)
+    float* handed = reinterpret_cast<float*>(keys);
+    if (group[tid] >= t) {
+      const int at = atomicAdd(&givers, 1);
+      giver[at] = tid;
+#pragma unroll
+      for (int e = 0; e < E; ++e) handed[at * E + e] = v[e];
+    }
+    __syncthreads();
+    const int all = __builtin_amdgcn_readfirstlane(givers * E);
+    float y[kMaxTop * E / kThreads];
+#pragma unroll
+    for (int k = 0; k < kMaxTop * E / kThreads; ++k) {
+      if (k * kThreads >= all) break;
+      y[k] = handed[min(k * kThreads + tid, all - 1)];
+    }
+    __syncthreads();  // the keys take the logits' place
+#pragma unroll
+    for (int k = 0; k < kMaxTop * E / kThreads; ++k) {
+      if (k * kThreads >= all) break;
+      const int i = k * kThreads + tid;
+      if (i < all && !(y[k] < tv)) {
+        const int id = place_of(giver[i / E], i % E);
+        const uint64_t key = key_of<T>(y[k], id);
+        if (id >= 0 && id < a.vocab && key >= t) keys[atomicAdd(&found, 1)] = key;
+      }
+    }
+    __syncthreads();
+    rank_first(keys, found, n, first);
     __syncthreads();
   }
 
@@ -222,19 +304,19 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
       const int all = a.chunks * n, few = min(n, (n - 1) / a.chunks + 2);  // at most 64 + 2 * 65 words
       uint64_t* left = keys + all;
       __syncthreads();
-      if (tid == 0) top.found = 0;
+      if (tid == 0) found = 0;
       if (wid == 0) {
         const auto key = [&](int i) { return keys[i / few * n + i % few]; };
         const uint64_t t = a.chunks * few <= kWave ? nth_largest<T, 1>(key, a.chunks * few, n)
                                                    : nth_largest<T, 4>(key, a.chunks * few, n);
-        if (lane == 0) top.threshold = t;
+        if (lane == 0) threshold = t;
       }
       __syncthreads();
-      const uint64_t t = top.threshold;
+      const uint64_t t = threshold;
       for (int i = tid; i < all; i += kThreads)
-        if (keys[i] >= t) left[atomicAdd(&top.found, 1)] = keys[i];
+        if (keys[i] >= t) left[atomicAdd(&found, 1)] = keys[i];
       __syncthreads();
-      rank_first(left, top.found, n, first);
+      rank_first(left, found, n, first);
       __syncthreads();
     }
   }

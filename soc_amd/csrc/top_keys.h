@@ -113,103 +113,5 @@ __device__ __forceinline__ void rank_first(const uint64_t* keys, int count, int 
   }
 }
 
-// LDS of block_first. found and givers are 0 before it, with a barrier since.
-struct BlockTop {
-  uint64_t group[kThreads];
-  uint64_t threshold;
-  int giver[kMaxTop];
-  int found, givers, tied;
-};
-// The n first tokens of a block's chunk, in order, to `first` (0 where it has fewer; a barrier before it is read), by all
-// threads. A thread holds E logits v, logit e of id place(e) (of another thread: place_of(thread, e)), its largest `best`;
-// ids outside [0, vocab) are no tokens and their logits -inf. keys: n * E words of LDS. Each thread's largest token stands
-// for its E: the n-th largest of those keys is a threshold that at most n threads reach, so at most n E tokens (64 of
-// normal data) are candidates, and those rank each other. No step depends on how many values are equal. nans: whether a NaN
-// may be among the logits.
-template <typename T, int E, typename Place, typename PlaceOf>
-__device__ __forceinline__ void block_first(const float (&v)[E], float best, bool nans, Place place, PlaceOf place_of,
-                                            int vocab, int n, uint64_t* keys, BlockTop& sh, uint64_t* first) {
-  constexpr int kLow = sizeof(T) == 2 ? 16 : 0;  // lowest bit of an order
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
-  // the order of the thread's largest; 0 where it has no logit (the lowest of its ids is place(0), or 0). Where the sum
-  // is NaN, a NaN may hide from `best`
-  uint32_t order = place(0) < vocab ? order_of<T>(best) : 0;
-  if (nans) {
-    order = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (place(e) >= 0 && place(e) < vocab) order = max(order, order_of<T>(v[e]));
-  }
-  sh.group[tid] = static_cast<uint64_t>(order) << 32;
-  __syncthreads();
-  uint32_t w[kThreads / kWave];  // wave 0
-  if (wid == 0) {
-#pragma unroll
-    for (int j = 0; j < kThreads / kWave; ++j) w[j] = static_cast<uint32_t>(sh.group[j * kWave + lane] >> 32);
-    bool exact;
-    const uint32_t o = nth_word(w, n, kLow, &exact);
-    if (lane == 0) {
-      sh.threshold = static_cast<uint64_t>(o) << 32;
-      sh.tied = !exact && o != 0;
-    }
-  }
-  __syncthreads();
-  if (sh.tied) {  // threads whose largest are equal at the threshold: those of the lowest ids
-    const uint32_t o = static_cast<uint32_t>(sh.threshold >> 32);
-    if (order == o) {
-      const float ov = value_of<T>(o);
-      int id = 0;
-#pragma unroll
-      for (int e = E - 1; e >= 0; --e)
-        if ((v[e] == ov || (v[e] != v[e] && ov != ov)) && place(e) >= 0 && place(e) < vocab) id = place(e);
-      sh.group[tid] |= low_of(id);
-    }
-    __syncthreads();
-    if (wid == 0) {
-      const int ties = n - reaching(w, o + 1);
-#pragma unroll
-      for (int j = 0; j < kThreads / kWave; ++j)
-        w[j] = w[j] == o ? static_cast<uint32_t>(sh.group[j * kWave + lane]) : 0;
-      bool exact;
-      const uint32_t low = nth_word(w, ties, 0, &exact);
-      if (lane == 0) sh.threshold |= low;
-    }
-  }
-  if (tid < n) first[tid] = 0;
-  __syncthreads();
-  const uint64_t t = max(sh.threshold, uint64_t{1});
-  const float tv = value_of<T>(static_cast<uint32_t>(t >> 32));
-  // the logits of the threads that reach it, at most n, are handed to all threads: E registers tested in place would be
-  // E copies of what follows, mostly skipped (one row top 20 11.6 us for 10.7, 777 fp16 rows 91 for 87)
-  float* handed = reinterpret_cast<float*>(keys);
-  if (sh.group[tid] >= t) {
-    const int at = atomicAdd(&sh.givers, 1);
-    sh.giver[at] = tid;
-#pragma unroll
-    for (int e = 0; e < E; ++e) handed[at * E + e] = v[e];
-  }
-  __syncthreads();
-  const int all = __builtin_amdgcn_readfirstlane(sh.givers * E);
-  float y[kMaxTop * E / kThreads];
-#pragma unroll
-  for (int k = 0; k < kMaxTop * E / kThreads; ++k) {
-    if (k * kThreads >= all) break;
-    y[k] = handed[min(k * kThreads + tid, all - 1)];
-  }
-  __syncthreads();  // the keys take the logits' place
-#pragma unroll
-  for (int k = 0; k < kMaxTop * E / kThreads; ++k) {
-    if (k * kThreads >= all) break;
-    const int i = k * kThreads + tid;
-    if (i < all && !(y[k] < tv)) {
-      const int id = place_of(sh.giver[i / E], i % E);
-      const uint64_t key = key_of<T>(y[k], id);
-      if (id >= 0 && id < vocab && key >= t) keys[atomicAdd(&sh.found, 1)] = key;
-    }
-  }
-  __syncthreads();
-  rank_first(keys, sh.found, n, first);
-}
-
 }  // namespace
 }  // namespace soc
