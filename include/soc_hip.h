@@ -493,6 +493,23 @@ int soc_paged_compact(soc_ctx* ctx, int32_t n, const int32_t* lens, int32_t page
                       int32_t* new_ring, int32_t num_pages, const int64_t* cursors, int32_t* moves, int32_t max_moves,
                       int32_t* move_count, int32_t* status);
 
+/* soc_paged_attention_decode for sequences of which groups begin alike: group g is rows group_starts[g] .. group_starts[g + 1]
+ * - 1 (device memory, groups + 1 entries, ascending; rows of no group stand for themselves), and the first prefix_lens[g]
+ * positions of its rows hold the same keys and values, as a rule because they name the same pages. Those positions may be
+ * read once for all the group's rows, from any of their pages; the rest from each row's own. That they are the same is the
+ * caller's word. For the rest the groups are a hint: starts that do not ascend within the n rows, prefixes that are negative,
+ * longer than a row or than max_prefix, rows beyond max_group in a group, prefixes too short to be worth it: then a row's
+ * keys are read from its own pages. 1 <= groups <= 4096; 1 <= max_group <= n rows of a group and 0 <= max_prefix <= max_pages *
+ * page_size positions set what is launched; with groups of max_group > 1 and long prefixes that is groups * (max_group *
+ * q_heads / 32 + kv_heads) blocks at least, at most 2^23.
+ * Everything else as there; a row's bits follow also from its group's size and prefix and from its place in it, not from
+ * the other rows' lengths or contents. A page outside the cache within the prefix makes all rows that read it NaN. */
+int soc_paged_attention_shared(soc_ctx* ctx, const soc_paged_cache* cache, const void* q, int64_t q_stride, int32_t dtype,
+                               const int32_t* block_table, int64_t table_stride, int32_t max_pages,
+                               const int32_t* seq_lens, int32_t n, const int32_t* group_starts,
+                               const int32_t* prefix_lens, int32_t groups, int32_t max_group, int32_t max_prefix,
+                               int32_t q_heads, float scale, void* out, int64_t out_stride, float* lse);
+
 /* ---- seeded synthetic data (this project's generator; the reference has none) ---- */
 int soc_synth_normal_f16(uint64_t seed, const char* name, float sigma, int64_t offset, int64_t n, uint16_t* out);
 int soc_synth_uniform_f16(uint64_t seed, const char* name, float lo, float hi, int64_t offset, int64_t n,

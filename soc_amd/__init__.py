@@ -9,5 +9,5 @@ from .capi import (  # noqa: F401
     attention_decode, attention_prefill, decode_steps, decode_steps_noalloc, dequant, forward, gemm_f16, gemv_f16,
     lib, load_bundle, prefill, qmm, quantize_group, sample_topk, synth_codes, synth_int_uniform, synth_normal_f16, synth_tokens, synth_uniform_f16,
     synth_weights, tensor_specs, PagedCache, Rope, logprobs, paged_append, paged_attention_decode, paged_plan,
-    PagedLayers, beam_select, paged_compact, paged_copy, paged_fork,
+    PagedLayers, beam_select, paged_attention_shared, paged_compact, paged_copy, paged_fork,
 )

@@ -202,6 +202,8 @@ def lib() -> C.CDLL:
         "soc_paged_fork": (C.c_int, [P, I32, P, P, P, I32, P, P, I32, I64, P, I32, P, P, P, P, P, P, P]),
         "soc_paged_copy": (C.c_int, [P, P, I32, P, P, I32]),
         "soc_paged_compact": (C.c_int, [P, I32, P, I32, P, P, I32, I64, P, P, I32, P, P, I32, P, P]),
+        "soc_paged_attention_shared": (C.c_int, [P, P, P, I64, I32, P, I64, I32, P, I32, P, P, I32, I32, I32, I32, F32, P,
+                                                 I64, P]),
         "soc_synth_normal_f16": (C.c_int, [U64, C.c_char_p, F32, I64, I64, P]),
         "soc_synth_uniform_f16": (C.c_int, [U64, C.c_char_p, F32, F32, I64, I64, P]),
         "soc_synth_tokens": (C.c_int, [U64, C.c_char_p, I32, I64, P]),
@@ -766,3 +768,12 @@ def paged_compact(ctx: Context, n: int, lens: int, page_size: int, block_table: 
                   max_moves: int, move_count: int, status: int) -> None:
     check(lib().soc_paged_compact(ctx.h, n, lens, page_size, block_table, new_table, max_pages, table_stride, free_ring,
                                   new_ring, num_pages, cursors, moves, max_moves, move_count, status))
+
+
+def paged_attention_shared(ctx: Context, cache: PagedCache, q: int, q_stride: int, dtype: str, block_table: int,
+                           table_stride: int, max_pages: int, seq_lens: int, n: int, group_starts: int,
+                           prefix_lens: int, groups: int, max_group: int, max_prefix: int, q_heads: int, scale: float,
+                           out: int, out_stride: int, lse: int | None = None) -> None:
+    check(lib().soc_paged_attention_shared(ctx.h, cache.ref, q, q_stride, DTYPES[dtype], block_table, table_stride,
+                                           max_pages, seq_lens, n, group_starts, prefix_lens, groups, max_group,
+                                           max_prefix, q_heads, scale, out, out_stride, lse))

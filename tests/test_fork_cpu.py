@@ -90,3 +90,23 @@ def test_beam_refusals(kw, text):
     refused(lib().soc_beam_select(None, SOME, a["dtype"], a["vocab"], a["groups"], a["beams"], a["vocab"], a["temperature"],
                                   SOME, a["stop_p"], a["stops"], a["top"], SOME, SOME, SOME, a["next"], a["next"],
                                   a["next"]), text)
+
+
+@pytest.mark.parametrize("kw,text", [
+    ({"dtype": 2}, "dtype"), ({"n": 0}, "65535 sequences"), ({"n": 65536, "groups": 1}, "65535 sequences"),
+    ({"max_pages": 0}, "max_pages"), ({"max_pages": 1 << 27}, "max_pages"), ({"groups": 0}, "groups"),
+    ({"groups": 5}, "groups"), ({"n": 5000, "groups": 4097}, "groups"), ({"max_group": 0}, "max_group"),
+    ({"max_group": 5}, "max_group"), ({"max_prefix": -1}, "max_prefix"), ({"max_prefix": 129}, "max_prefix"),
+    ({"q_heads": 0}, "query heads"), ({"q_heads": 5}, "query heads"), ({"q_heads": 34}, "query heads"),
+    ({"scale": float("inf")}, "scale"), ({"out": SOME, "out_stride": 513}, "in place"),
+    ({"cache": cache(page_size=8)}, "page_size"), ({"cache": None}, "null paged cache"),
+    ({"cache": cache(kv_heads=1024), "q_heads": 1024, "n": 1025}, "2^20"), ({}, "null context"),
+])
+def test_shared_attention_refusals(kw, text):
+    a = dict(cache=cache(), dtype=0, max_pages=8, n=4, groups=2, max_group=4, max_prefix=128, q_heads=4, scale=0.0,
+             out=2 * SOME, out_stride=512)
+    a.update(kw)
+    refused(lib().soc_paged_attention_shared(None, C.byref(a["cache"]) if a["cache"] else None, SOME, 512, a["dtype"], SOME,
+                                             a["max_pages"], a["max_pages"], SOME, a["n"], SOME, SOME, a["groups"],
+                                             a["max_group"], a["max_prefix"], a["q_heads"], a["scale"], a["out"],
+                                             a["out_stride"], SOME), text)
