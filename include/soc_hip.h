@@ -499,9 +499,8 @@ int soc_paged_compact(soc_ctx* ctx, int32_t n, const int32_t* lens, int32_t page
  * read once for all the group's rows, from any of their pages; the rest from each row's own. That they are the same is the
  * caller's word. For the rest the groups are a hint: starts that do not ascend within the n rows, prefixes that are negative,
  * longer than a row or than max_prefix, rows beyond max_group in a group, prefixes too short to be worth it: then a row's
- * keys are read from its own pages. 1 <= groups <= 4096; 1 <= max_group <= n rows of a group and 0 <= max_prefix <= max_pages *
- * page_size positions set what is launched; with groups of max_group > 1 and long prefixes that is groups * (max_group *
- * q_heads / 32 + kv_heads) blocks at least, at most 2^23.
+ * keys are read from its own pages. 1 <= groups <= 4096, no more than n. max_group (at least 1) and max_prefix (at least 0)
+ * bound what is launched.
  * Everything else as there; a row's bits follow also from its group's size and prefix and from its place in it, not from
  * the other rows' lengths or contents. A page outside the cache within the prefix makes all rows that read it NaN. */
 int soc_paged_attention_shared(soc_ctx* ctx, const soc_paged_cache* cache, const void* q, int64_t q_stride, int32_t dtype,

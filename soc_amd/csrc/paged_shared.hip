@@ -33,7 +33,7 @@ struct SharedArgs {
   int64_t out_stride;
   float* lse;
   bool wide_q;  // query rows are 32-byte aligned (16 in fp16): eight values a load
-  int tiles;    // blocks for the columns of a group
+  int columns, tiles;  // columns of a block; blocks for the columns of a group
   int prefix_splits, prefix_grid, prefix_blocks;
   int splits, grid, most;
   float* part;   // [n][nkv][prefix_grid + grid][group * (HD + 2)]: outputs, then maxima, then sums
@@ -44,6 +44,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kWeightBits = 14.0f;  // weights are held times 2^14
 constexpr int kPrefixMost = 1024;     // keys of a prefix a block takes, where there are blocks enough
 constexpr int kTile = 32;             // keys a wave takes at a time
+constexpr int kNarrow = 16, kWide = 64;  // columns of a block
+constexpr float kWideBits = 10.0f, kLazy = 4.0f;  // weights of a reference that may be 2^4 too low
 
 // Reduces over the four lanes l % 16 + {0, 16, 32, 48}; every lane gets the result.
 template <typename F>
@@ -271,6 +273,176 @@ __device__ __forceinline__ bool attend(const SharedArgs& a, int g, const Columns
   return lost;
 }
 
+// A group's prefix for 64 columns, 16 for each of the four waves: the keys' 32-key tiles go through LDS, the next one on its
+// way while one is in use. A tile row's 16-byte chunk c lies at slot c ^ swizzle(row), so that 16 rows read at one chunk reach
+// all banks; ds_read_b64_tr_b16 gives V^T (in each 16-lane group, lane j names 4 dims of one key, and lane i receives dim i of
+// 4 keys). Tiles are whole. The running reference, weights 2^(t - m), follows a score only where that gives a weight above 2^14,
+// and then makes it 2^10, so that the sums are seldom rescaled. A weight's fp16 high part is cut off, the low part is the rest.
+template <int HD>
+struct WideShared {
+  f16 keys[2][kTile * HD], values[2][kTile * HD];
+};
+typedef __fp16 hv4 __attribute__((__vector_size__(4 * sizeof(__fp16))));  // what the transposing read gives
+template <int HD>
+__device__ __forceinline__ constexpr int swizzle(int row) {
+  return HD == 128 ? row & 15 : (row >> 1) & 7;
+}
+template <typename T, int HD>
+struct WideResult {
+  f32x4 o[HD / 16];  // dims 16 d + 4 (lane / 16) + r of column lane % 16
+  float m, l;
+  bool lost;
+};
+template <typename T, int HD>
+__device__ __forceinline__ WideResult<T, HD> attend_wide(const SharedArgs& a, int g, const Columns<T>& cols,
+                                                         WideShared<HD>& sh) {
+  constexpr int KC = HD / 32, ND = HD / 16;
+  constexpr int kChunks = HD / 8, kRows = 64 / kChunks;  // 16-byte chunks of a row; rows of a wave's load
+  constexpr int kLoads = 8 / kRows;                      // of a wave's 8 rows of a tile
+  constexpr bool kLow = sizeof(T) == 4;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, row = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tiles = static_cast<int>(cols.end - cols.begin) / kTile;
+  const uint32_t mask = (1u << a.page_shift) - 1;
+  WideResult<T, HD> out;
+  out.lost = false;
+  // a wave loads rows 8 wid .. 8 wid + 7 of a tile, which lie in its half wid / 2; lane l holds the page of that half of
+  // tile l (64 tiles ahead)
+  auto pages_from = [&](int first) {
+    const uint32_t key = min(cols.begin + (first + lane) * kTile + (wid >> 1) * 16, cols.end - 1);
+    const int page = checked_page(cols.table[key >> a.page_shift], a.num_pages);
+    out.lost |= page < 0;
+    return max(page, 0);
+  };
+  int pages = pages_from(0);
+  const f16* keys = a.keys + (static_cast<int64_t>(g) << a.page_shift) * HD;
+  const f16* values = a.values + (static_cast<int64_t>(g) << a.page_shift) * HD;
+  auto load_tile = [&](int i) {
+    const int64_t page = __builtin_amdgcn_readlane(pages, i & 63);
+    const uint32_t place = (cols.begin + i * kTile + (wid >> 1) * 16) & mask;
+    const int64_t at = page * a.page_stride + place * HD;
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const int first = 8 * wid + n * kRows, r = first + lane / kChunks;  // of the tile
+      const int off = (r & 15) * HD + ((lane % kChunks) ^ swizzle<HD>(r)) * 8;
+      __builtin_amdgcn_global_load_lds(keys + at + off, sh.keys[i & 1] + first * HD, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(values + at + off, sh.values[i & 1] + first * HD, 16, 0, 0);
+    }
+  };
+  load_tile(0);
+  const int mine = cols.count - wid * 16;  // columns of this wave
+  f16x8 qh[KC], ql[kLow ? KC : 1];
+  float to_log2;
+  {
+    const int at = cols.first + min(wid * 16 + col, cols.count - 1), r = at / cols.group;
+    const T* p = cols.q + r * cols.q_stride + (at - r * cols.group) * HD + row * 8;
+    float v[KC][8];
+    float big = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      if (a.wide_q) {
+        typedef T Q8 __attribute__((ext_vector_type(8)));
+        const Q8 x = *reinterpret_cast<const Q8*>(p + k * 32);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[k][i] = static_cast<float>(x[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[k][i] = static_cast<float>(p[k * 32 + i]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < KC; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(v[k][i]));
+    big = across_rows(big, [](float x, float y) { return fmaxf(x, y); });
+    const int exponent = static_cast<int>(__float_as_uint(big) >> 23);
+    const int e = big > 0.0f && exponent < 255 ? min(140 - exponent, 126) : 0;
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    to_log2 = fabsf(a.scale) * __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * kLog2e;
+    const float signed_up = copysignf(up, a.scale);  // so that larger sums are larger scores
+#pragma unroll
+    for (int k = 0; k < KC; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = v[k][i] * signed_up;
+        qh[k][i] = static_cast<f16>(x);
+        if constexpr (kLow) ql[k][i] = static_cast<f16>(x - static_cast<float>(qh[k][i]));
+      }
+  }
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < ND; ++d) out.o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  __syncthreads();  // tile 0 is there
+  for (int i = 0; i < tiles; ++i) {
+    if (i + 1 < tiles) {
+      if (((i + 1) & 63) == 0) pages = pages_from(i + 1);
+      load_tile(i + 1);
+    }
+    if (mine > 0) {
+      const f16* kt = sh.keys[i & 1];
+      const f16* vt = sh.values[i & 1];
+      f32x4 sc[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        sc[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int r = h * 16 + col;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          const f16x8 k = *reinterpret_cast<const f16x8*>(kt + r * HD + ((c * 4 + row) ^ swizzle<HD>(r)) * 8);
+          if constexpr (kLow) sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[c], sc[h], 0, 0, 0);
+          sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[c], sc[h], 0, 0, 0);
+        }
+      }
+      float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                        fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+      top = across_rows(top, [](float u, float v) { return fmaxf(u, v); }) * to_log2;
+      const bool moves = top - (kWideBits + kLazy) > m;
+      if (__ballot(moves) != 0) {
+        const float to = moves ? top - kWideBits : m, f = moves ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+        m = to;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) out.o[d][r] *= f;
+      }
+      f16x8 ph, pl;
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[j >> 2][j & 3], to_log2, -m));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[j >> 2][(j & 3) + 1], to_log2, -m));
+        l += p0 + p1;
+        const auto hv = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+        const auto lv = __builtin_amdgcn_cvt_pkrtz(fmaf(static_cast<float>(hv[0]), -1.0f, p0),
+                                                   fmaf(static_cast<float>(hv[1]), -1.0f, p1));
+        ph[j] = hv[0];
+        ph[j + 1] = hv[1];
+        pl[j] = lv[0];
+        pl[j + 1] = lv[1];
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        f16x8 v;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = h * 16 + row * 4 + (col >> 2), c = 2 * d + ((col & 3) >> 1);
+          const f16* at = vt + r * HD + (c ^ swizzle<HD>(r)) * 8 + (col & 1) * 4;
+          const hv4 w = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) hv4*)at);
+          const f16x4 u = __builtin_bit_cast(f16x4, w);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[4 * h + j] = u[j];
+        }
+        out.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, out.o[d], 0, 0, 0);
+        out.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, out.o[d], 0, 0, 0);
+      }
+    }
+    __syncthreads();  // tile i + 1 is there, and nobody needs tile i
+  }
+  out.m = m + kWeightBits;  // of weights held times 2^14, as the other parts' are
+  out.l = across_rows(l, [](float u, float v) { return u + v; });
+  return out;
+}
+
 // What a block finds out about the groups, in one trip: whether their starts ascend within the rows, and a group's bounds and
 // prefix. `row` >= 0: the group of that row (-1 if none), else group `want`.
 struct GroupOf {
@@ -304,12 +476,18 @@ __device__ __forceinline__ GroupOf group_of(const SharedArgs& a, int row, int wa
 }
 __device__ __forceinline__ int chunks_of(int keys, int chunk) { return keys <= 0 ? 0 : (keys - 1) / chunk + 1; }
 
-template <typename T, int HD, int NT>
-__global__ __launch_bounds__(256, 2) void k_shared(SharedArgs a) {
-  __shared__ AttendShared<T, HD, NT> sh;
+template <typename T, int HD>
+__global__ __launch_bounds__(256, 3) void k_shared(SharedArgs a) {
+  union Shared {
+    AttendShared<T, HD, 1> narrow;
+    WideShared<HD> wide;
+  };
+  __shared__ alignas(16) Shared lds;
   __shared__ int32_t found[4];
   __shared__ int leader;
-  __shared__ bool whole[16 * NT];  // whether a column's row holds the whole prefix
+  __shared__ bool whole[kWide];  // whether a column's row holds the whole prefix
+  __shared__ bool bad_page;
+  AttendShared<T, HD, 1>& sh = lds.narrow;
   const int tid = threadIdx.x, G = a.group;
   const int stride = G * (HD + 2), all = a.prefix_grid + a.grid;
   if (static_cast<int>(blockIdx.x) < a.prefix_blocks) {
@@ -324,11 +502,14 @@ __global__ __launch_bounds__(256, 2) void k_shared(SharedArgs a) {
     const int chunk = attention_chunk(of.prefix, a.prefix_splits, a.prefix_grid, kPrefixMost);
     const int c0 = s * chunk;
     Columns<T> cols;
-    cols.first = tile * 16 * NT;
-    cols.count = min(of.count * G - cols.first, 16 * NT);
+    cols.first = tile * a.columns;
+    cols.count = min(of.count * G - cols.first, a.columns);
     if (c0 >= of.prefix || cols.count <= 0) return;
     // pages are those of the first row that holds the whole prefix
-    if (tid == 0) leader = of.count;
+    if (tid == 0) {
+      leader = of.count;
+      bad_page = false;
+    }
     if (tid < cols.count)
       whole[tid] = checked_length(a.lens[of.first + (cols.first + tid) / G], a.max_pages, a.page_shift) >= of.prefix;
     __syncthreads();
@@ -345,7 +526,26 @@ __global__ __launch_bounds__(256, 2) void k_shared(SharedArgs a) {
     cols.table = a.table + (of.first + leader) * a.table_stride;
     cols.begin = c0;
     cols.end = min(of.prefix, c0 + chunk);
-    const bool lost = attend<T, HD, NT>(a, g, cols, sh);
+    if (a.columns == kWide) {
+      const WideResult<T, HD> x = attend_wide<T, HD>(a, g, cols, lds.wide);
+      if (x.lost) bad_page = true;
+      __syncthreads();
+      const int lane = tid & 63, row = lane >> 4, c = tid / 64 * 16 + (lane & 15);
+      if (c >= cols.count || !whole[c]) return;
+      const int at = cols.first + c, r = at / G, h = at - r * G;
+      float* part = a.part + (((of.first + r) * static_cast<int64_t>(a.nkv) + g) * all + s) * stride;
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; j += 2)
+          *reinterpret_cast<f32x2*>(part + h * HD + d * 16 + row * 4 + j) = f32x2{x.o[d][j], x.o[d][j + 1]};
+      if (row == 0) {
+        part[G * HD + h] = x.m;
+        part[G * HD + G + h] = bad_page ? __builtin_nanf("") : x.l;
+      }
+      return;
+    }
+    const bool lost = attend<T, HD, 1>(a, g, cols, sh);
     for (int i = tid; i < cols.count * (HD / 2); i += 256) {
       const int c = i / (HD / 2), d = (i - c * (HD / 2)) * 2, at = cols.first + c, r = at / G, h = at - r * G;
       if (!whole[c]) continue;  // reads all its keys by itself
@@ -388,7 +588,7 @@ __global__ __launch_bounds__(256, 2) void k_shared(SharedArgs a) {
   cols.table = a.table + b * a.table_stride;
   cols.begin = begin + c0;
   cols.end = min(len, begin + c0 + chunk);
-  const bool lost = attend<T, HD, NT>(a, g, cols, sh);
+  const bool lost = attend<T, HD, 1>(a, g, cols, sh);
   float* part = a.part + (pair * all + before + s) * stride;
   for (int i = tid; i < G * (HD / 2); i += 256) {
     const int c = i / (HD / 2), d = (i - c * (HD / 2)) * 2;
@@ -464,10 +664,7 @@ __global__ __launch_bounds__(256) void k_shared_join(SharedArgs a, int hd) {
 template <typename T, int HD>
 hipError_t launch_shared(const SharedArgs& a, hipStream_t s) {
   const uint32_t blocks = a.prefix_blocks + static_cast<uint32_t>(a.n) * a.nkv * a.grid;
-  if (a.tiles > 0 && a.max_group * a.group > 16)
-    hipLaunchKernelGGL((k_shared<T, HD, 2>), dim3(blocks), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((k_shared<T, HD, 1>), dim3(blocks), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((k_shared<T, HD>), dim3(blocks), dim3(256), 0, s, a);
   hipLaunchKernelGGL((k_shared_join<T>), dim3(static_cast<uint32_t>(a.n) * a.nkv), dim3(256), 0, s, a, HD);
   return hipGetLastError();
 }
@@ -495,10 +692,10 @@ int soc_paged_attention_shared(soc_ctx* ctx, const soc_paged_cache* cache, const
     return soc::fail(SOC_ERR_INVALID, "shared attention: need max_pages > 0 and max_pages * page_size up to 2^30");
   if (groups <= 0 || groups > n || groups > 4096)
     return soc::fail(SOC_ERR_INVALID, "shared attention: 1 to 4096 groups, no more than sequences");
-  if (max_group <= 0 || max_group > n)
-    return soc::fail(SOC_ERR_INVALID, "shared attention: max_group must be 1 to n");
-  if (max_prefix < 0 || max_prefix > max_pages * cache->page_size)
-    return soc::fail(SOC_ERR_INVALID, "shared attention: max_prefix must be 0 to max_pages * page_size");
+  if (max_group <= 0 || max_prefix < 0)
+    return soc::fail(SOC_ERR_INVALID, "shared attention: need max_group > 0 and max_prefix >= 0");
+  max_group = std::min(max_group, n);
+  max_prefix = std::min(max_prefix, max_pages * cache->page_size);
   if (q_heads <= 0 || q_heads % cache->kv_heads != 0 || q_heads / cache->kv_heads > 16)
     return soc::fail(SOC_ERR_INVALID, "shared attention: query heads per KV head must be 1 to 16");
   if (!std::isfinite(scale)) return soc::fail(SOC_ERR_INVALID, "shared attention: scale must be finite");
@@ -549,8 +746,8 @@ int soc_paged_attention_shared(soc_ctx* ctx, const soc_paged_cache* cache, const
   const int64_t room = std::max<int64_t>(2, (int64_t{512} << 20) / static_cast<int64_t>(pairs * part));
   const bool share = max_group > 1 && max_prefix >= 4 * soc::kTile;
   if (share) {
-    const int columns = max_group * a.group > 16 ? 32 : 16;
-    a.tiles = (max_group * a.group + columns - 1) / columns;
+    a.columns = max_group * a.group > soc::kNarrow ? soc::kWide : soc::kNarrow;
+    a.tiles = (max_group * a.group + a.columns - 1) / a.columns;
     const int64_t units = static_cast<int64_t>(groups) * a.nkv * a.tiles;
     a.prefix_splits = static_cast<int>(std::min<int64_t>(32, (256 + units - 1) / units));
     a.prefix_grid = static_cast<int>(

@@ -96,7 +96,7 @@ def test_beam_refusals(kw, text):
     ({"dtype": 2}, "dtype"), ({"n": 0}, "65535 sequences"), ({"n": 65536, "groups": 1}, "65535 sequences"),
     ({"max_pages": 0}, "max_pages"), ({"max_pages": 1 << 27}, "max_pages"), ({"groups": 0}, "groups"),
     ({"groups": 5}, "groups"), ({"n": 5000, "groups": 4097}, "groups"), ({"max_group": 0}, "max_group"),
-    ({"max_group": 5}, "max_group"), ({"max_prefix": -1}, "max_prefix"), ({"max_prefix": 129}, "max_prefix"),
+    ({"max_group": -2}, "max_group"), ({"max_prefix": -1}, "max_prefix"), ({"max_prefix": 129, "max_group": 5}, "null context"),
     ({"q_heads": 0}, "query heads"), ({"q_heads": 5}, "query heads"), ({"q_heads": 34}, "query heads"),
     ({"scale": float("inf")}, "scale"), ({"out": SOME, "out_stride": 513}, "in place"),
     ({"cache": cache(page_size=8)}, "page_size"), ({"cache": None}, "null paged cache"),
