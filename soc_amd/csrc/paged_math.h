@@ -53,6 +53,31 @@ SOC_HD int32_t attention_chunk(int32_t len, int32_t splits, int32_t grid, int32_
   return chunk == 128 && len > 16 * 128 ? 256 : chunk;
 }
 
+// How keys are split over waves or blocks: `splits` chunks where none would be longer than `most` keys, multiples of that
+// where there are more keys, at most `grid` chunks; chunks of whole `least` keys (a multiple of 32).
+struct Chunks {
+  int32_t splits, grid, least, most;
+};
+SOC_HD int32_t chunk_of(int32_t keys, const Chunks& c) {
+  if (keys <= 0) return c.least;
+  int32_t want = ((keys - 1) / c.most / c.splits + 1) * c.splits;
+  want = want < c.grid ? want : c.grid;
+  return ((keys - 1) / want / c.least + 1) * c.least;
+}
+SOC_HD int32_t chunks_of(int32_t keys, int32_t chunk) { return keys <= 0 ? 0 : (keys - 1) / chunk + 1; }
+// For `units` times up to `longest` keys (>= 1): enough chunks for `waves` of them at a time, no more than `room` a unit.
+SOC_HD Chunks chunks_for(int64_t units, int64_t longest, int32_t waves, int32_t least, int32_t most, int32_t room) {
+  Chunks c{1, 1, least, most};
+  const int64_t splits = (waves + units - 1) / units;
+  c.splits = static_cast<int32_t>(splits < room ? splits : room);
+  const int64_t grid = ((longest - 1) / most / c.splits + 1) * c.splits, fit = (longest + least - 1) / least;
+  const int64_t several = 8 * static_cast<int64_t>(waves) / units;  // of large batches' long rows
+  int64_t g = grid < fit ? grid : fit;
+  g = g < (several > 8 ? several : 8) ? g : (several > 8 ? several : 8);
+  c.grid = static_cast<int32_t>(g < room ? g : room);
+  return c;
+}
+
 // Place of a cursor in a ring of `size` entries, for any cursor.
 SOC_HD int32_t ring_place(int64_t cursor, int32_t size) {
   return static_cast<int32_t>(static_cast<uint64_t>(cursor) % static_cast<uint64_t>(size));

@@ -19,6 +19,12 @@ pytestmark = pytest.mark.gpu
 INF = np.inf
 
 
+@pytest.fixture(autouse=True)
+def shared(monkeypatch):
+    """Small batches would be read row by row."""
+    monkeypatch.setenv("SOC_PAGED_SHARED", "always")
+
+
 def formula(q, k, v, scale):
     """q [nq][hd], k / v [nkv][len][hd] -> (out, lse, tolerances) in 64 bits."""
     nq, hd = q.shape
@@ -302,6 +308,28 @@ def test_agrees_with_the_unshared_one(gpu_ctx):
     for i in range(b.n):
         _, _, tol, _ = formula(q[i], *b.rows[i], 1 / math.sqrt(128))
         assert (np.abs(out[i] - other[i]) <= 2 * tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_little_to_read(gpu_ctx, dtype, monkeypatch):
+    """A small batch is answered as soc_paged_attention_decode answers it; a prefix as long as the rows, and one row."""
+    monkeypatch.delenv("SOC_PAGED_SHARED")
+    b = Batch([7, 3], [900, 333], [4, 0, 20, 33, 1, 100, 3, 50, 0, None], 16, 4, 128, 32)
+    out, _ = b.check(gpu_ctx, dtype)
+    with Arrays(gpu_ctx) as mem:
+        q = b.q.astype(NP[dtype])
+        pk, pv, po = mem.up(b.pool[0]), mem.up(b.pool[1]), mem.up(np.zeros_like(q))
+        S.paged_attention_decode(gpu_ctx, S.PagedCache(pk, pv, b.pages, 32, 4, 128), mem.up(q), 16 * 128, dtype, mem.up(b.table),
+                                 b.width, b.width, mem.up(b.lens.astype(np.int32)), b.n, 16, 0.0, po, 16 * 128)
+        assert np.array_equal(mem.down(po).reshape(out.shape), out)
+    Batch([1], [300], [5], 4, 2, 64, 16).check(gpu_ctx, dtype)
+
+
+def test_more_than_little_to_read(gpu_ctx, monkeypatch):
+    """The same rule from the other side."""
+    monkeypatch.delenv("SOC_PAGED_SHARED")
+    b = Batch([20, 4], [1100, 500], [7] * 24, 16, 8, 128, 64)
+    b.check(gpu_ctx)
 
 
 def test_refusals(gpu_ctx):
