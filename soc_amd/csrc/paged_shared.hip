@@ -7,9 +7,9 @@
 // 2^(t - m) (t: scores in base 2) and the sum of the weighted values; a second launch joins the parts of each (sequence, KV
 // head). (Joined by the last block to add one, a prefix's blocks have up to 16 of them to join one after the other: 16 groups
 // of 4 rows, 2000 common keys, took 100 us for 34.) Two ways to a part:
-//   a row's own keys, and a prefix of up to 16 columns: four waves take the 32-key tiles of a chunk in turn, all with the same
+//   a row's own keys, and up to 16 columns of a prefix: four waves take the 32-key tiles of a chunk in turn, all with the same
 //   columns, and add up their sums in LDS;
-//   a prefix of more columns: four waves with 16 columns each, whose key tiles go through LDS.
+//   up to 64 columns of a prefix: four waves with 16 columns each, whose key tiles go through LDS.
 // Keys and values are matrix operands as they come from memory:
 //   scores  S [16 keys][16 columns] = K . Q^T, v_mfma_f32_16x16x32_f16: lane l holds 8 dims of key l % 16, and of column
 //           l % 16. An fp32 query is an fp16 high part and what fp32 has beyond it, both added into one sum.
@@ -456,8 +456,9 @@ __device__ __forceinline__ GroupOf group_of(const SharedArgs& a, int row, int wa
       }
     }
   }
-  // a group of one, a short prefix, and rows beyond max_group: all keys are the row's own
-  if (__ballot(bad) != 0 || g.count < 2 || g.prefix < kShortest || (row >= 0 && row >= g.first + g.count))
+  // a short prefix, and rows beyond max_group: all keys are the row's own. (A group of one shares nothing, but its prefix has
+  // blocks, where a row's own keys have few)
+  if (__ballot(bad) != 0 || g.count < 1 || g.prefix < kShortest || (row >= 0 && row >= g.first + g.count))
     return GroupOf{0, 0, 0};
   return g;
 }
@@ -535,15 +536,18 @@ __device__ __forceinline__ void prefix_part(const SharedArgs& a, int unit, char*
   cols.end = min(of.prefix, c0 + chunk);
   Sums<HD> sums;
   bool lost;
-  if constexpr (kColumns == kMany) lost = attend_block<T, HD>(a, g, cols, lds, sums);
-  else lost = attend_wave<T, HD, false>(a, g, cols, sums);
+  const bool many = kColumns == kMany && cols.count > kFew;
+  if constexpr (kColumns == kMany) {
+    if (many) lost = attend_block<T, HD>(a, g, cols, lds, sums);
+  }
+  if (!many) lost = attend_wave<T, HD, false>(a, g, cols, sums);
   lost = __syncthreads_or(lost) != 0;
   const float nan = __builtin_nanf("");
   const auto part_of = [&](int r) {
     return a.part + (((of.first + r) * static_cast<int64_t>(a.nkv) + g) * a.most + s) * a.stride;
   };
   // not for a row that does not hold the prefix: it reads all its keys by itself
-  if constexpr (kColumns == kMany) {
+  if (many) {
     typedef float Four __attribute__((ext_vector_type(4), aligned(8)));
     const int c = wid * 16 + (lane & 15), at = cols.first + c, r = at / G, h = at - r * G, row = lane >> 4;
     if (c >= cols.count || !holds(r)) return;
