@@ -86,7 +86,7 @@ class Operands {
     const char *begin, *end;
   };
   const soc_ctx* ctx_;
-  Range known_[8];
+  Range known_[32];
   int count_ = 0;
 };
 

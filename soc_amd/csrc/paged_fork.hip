@@ -14,7 +14,8 @@ namespace {
 // ---- fork ------------------------------------------------------------------------------------------------------------
 // Whether a page is still named is found from the tables alone: no counts are kept that could go wrong. Each page has a
 // 64-bit word that outlives the call; its upper 48 bits are the call that wrote it last, so that nothing is cleared. Every
-// entry of the new table raises its page's word to (call, all ones); every entry that a row loses (its old page at a place
+// entry of the new table (but where the row before has the same page, which is then marked already) raises its page's word to
+// (call, all ones); every entry that a row loses (its old page at a place
 // where its new one is another, or none) raises it to (call, row + 1). Afterwards (call, row + 1) stands exactly at the pages
 // that no row names any more, with the last row that lost them; that row's entry puts the page into the ring. Maxima do not
 // depend on order.
@@ -147,13 +148,14 @@ __device__ __forceinline__ int fork_rows(const ForkArgs& a, Rows& s, int64_t hea
   return status;
 }
 
-// Row i's page at place j before and after; -1 where it has none there.
+// Row i's page at place j before and after; -1 where it has none there. `marked`: the row before has the same page after.
 struct ForkEntry {
   int32_t was, is;
+  bool marked;
 };
 template <typename Rows>
 __device__ __forceinline__ ForkEntry fork_entry(const ForkArgs& a, const Rows& s, int i, int j, int32_t head0) {
-  ForkEntry e{-1, -1};
+  ForkEntry e{-1, -1, false};
   const bool had = j < s.held[i], has = j < s.pages[i];
   const int p = s.parent[i];
   if (had) e.was = a.table[i * a.table_stride + j];
@@ -161,6 +163,7 @@ __device__ __forceinline__ ForkEntry fork_entry(const ForkArgs& a, const Rows& s
     const int t = s.take[i];
     if (t >= 0 && j == s.pages[i] - 1) e.is = a.ring[ring_place(head0, t, a.num_pages)];
     else e.is = p == i ? e.was : a.table[p * a.table_stride + j];
+    if (i > 0 && j < s.pages[i - 1] - (s.take[i - 1] >= 0)) e.marked = a.table[s.parent[i - 1] * a.table_stride + j] == e.is;
   }
   return e;
 }
@@ -171,7 +174,7 @@ __device__ __forceinline__ bool fork_mark(const ForkArgs& a, const Rows& s, int 
                                           uint64_t call) {
   if (j < s.pages[i]) {
     a.new_table[i * a.table_stride + j] = e.is;
-    if (call != 0 && checked_page(e.is, a.num_pages) >= 0)
+    if (call != 0 && !e.marked && checked_page(e.is, a.num_pages) >= 0)
       atomicMax(reinterpret_cast<unsigned long long*>(a.marks + e.is),
                 static_cast<unsigned long long>(call << 16 | 0xffffu));
   }
