@@ -241,16 +241,17 @@ __global__ __launch_bounds__(kSmallThreads) void k_fork_small(ForkArgs a) {
 
 // Large tables in three launches: marks; the pages for the ring, by row and chunk of columns; their places in the ring.
 template <int kEach>
-__global__ __launch_bounds__(kForkThreads) void k_fork_mark(ForkArgs a) {
-  __shared__ ForkRows<kEach * kForkThreads, kForkThreads / kWave> s;
+__global__ __launch_bounds__(kSmallThreads) void k_fork_mark(ForkArgs a) {
+  __shared__ ForkRows<kEach * kSmallThreads, kSmallThreads / kWave> s;
   const int64_t head = a.cursors_in[0], tail = a.cursors_in[1];
   const int32_t head0 = ring_place(head, a.num_pages);
   const uint64_t number = *a.call;
   int copies;
-  const int status = fork_rows<kEach, kForkThreads>(a, s, head, tail, blockIdx.x == 0, &copies);
+  const int status = fork_rows<kEach, kSmallThreads>(a, s, head, tail, blockIdx.x == 0, &copies);
   const uint64_t call = status == 0 ? number : 0;
-  for (int u = blockIdx.x; u < a.n * a.chunks; u += gridDim.x) {
-    const int i = u / a.chunks, j = (u - i * a.chunks) * kForkThreads + threadIdx.x;
+  constexpr int kUnits = kSmallThreads / kForkThreads;  // of a block at a time
+  for (int u = blockIdx.x * kUnits + threadIdx.x / kForkThreads; u < a.n * a.chunks; u += gridDim.x * kUnits) {
+    const int i = u / a.chunks, j = (u - i * a.chunks) * kForkThreads + threadIdx.x % kForkThreads;
     if (j < max(s.held[i], s.pages[i])) fork_mark(a, s, i, j, fork_entry(a, s, i, j, head0), call);
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -627,9 +628,9 @@ int soc_paged_fork(soc_ctx* ctx, int32_t n, const int32_t* parents, const int32_
   a.found = reinterpret_cast<int64_t*>(ctx->serve_ws);
   a.lost = reinterpret_cast<int32_t*>(ctx->serve_ws + 64);
   a.lost_count = reinterpret_cast<int32_t*>(ctx->serve_ws + 64 + lists);
-  const int blocks = std::min(units, 512);
-  auto* mark = n <= 4 * soc::kForkThreads ? soc::k_fork_mark<4> : soc::k_fork_mark<16>;
-  hipLaunchKernelGGL(mark, dim3(blocks), dim3(soc::kForkThreads), 0, ctx->stream, a);
+  const int blocks = std::min((units + 3) / 4, 256);
+  auto* mark = n <= soc::kSmallThreads ? soc::k_fork_mark<1> : soc::k_fork_mark<4>;
+  hipLaunchKernelGGL(mark, dim3(blocks), dim3(soc::kSmallThreads), 0, ctx->stream, a);
   hipLaunchKernelGGL(soc::k_fork_find, dim3(std::min(units, 2048)), dim3(soc::kForkThreads), 0, ctx->stream, a);
   hipLaunchKernelGGL(soc::k_fork_give, dim3(std::min(units, 256)), dim3(soc::kForkThreads), 0, ctx->stream, a);
   return soc::hip_status(hipGetLastError(), "paged fork");
