@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256) void k_paged_copy(CopyArgs a) {
 }
 
 // ---- compact ---------------------------------------------------------------------------------------------------------
-constexpr int kCompactThreads = 1024, kCompactPages = 1 << 20;
+constexpr int kCompactThreads = 1024, kCompactPages = 1 << 20, kAlonePages = 1 << 17;
 struct CompactArgs {
   int n;
   const int32_t* lens;
@@ -415,7 +415,9 @@ __global__ __launch_bounds__(256) void k_compact_mark(CompactArgs a) {
 }
 
 // Every block holds the whole bitmap and the counts of its groups of words in LDS, and answers for its share of the pages and
-// of the table's entries where each goes.
+// of the table's entries where each goes. kAlone: it forms the bitmap itself, else k_compact_mark has. (2000 pages
+// 8.5 us a call so, 11.7 in two launches; 131072 pages 15.6 both ways, each block reading 43000 entries of the ring.)
+template <bool kAlone>
 __global__ __launch_bounds__(kCompactThreads) void k_compact_apply(CompactArgs a) {
   extern __shared__ uint32_t words[];
   __shared__ int32_t counts[kCompactThreads + 1];
@@ -428,8 +430,23 @@ __global__ __launch_bounds__(kCompactThreads) void k_compact_apply(CompactArgs a
   int shift = 0;
   while ((kCompactThreads << shift) < a.words_count) ++shift;
   const int room = kCompactThreads << shift;
-  for (int w = tid; w < room; w += kCompactThreads) words[w] = w < a.words_count ? a.words[w] : 0;
   bool bad = false;
+  if constexpr (kAlone) {
+    for (int w = tid; w < room; w += kCompactThreads) words[w] = 0;
+    __syncthreads();
+    const int entries = good_cursors(head, tail, a.num_pages) ? static_cast<int>(tail - head) : 0;
+    for (int i0 = tid; i0 < entries; i0 += 8 * kCompactThreads) {
+      int32_t page[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) page[k] = a.ring[ring_place(head0, min(i0 + k * kCompactThreads, entries - 1), a.num_pages)];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i0 + k * kCompactThreads < entries && checked_page(page[k], a.num_pages) >= 0)
+          atomicOr(words + (page[k] >> 5), 1u << (page[k] & 31));
+    }
+  } else {
+    for (int w = tid; w < room; w += kCompactThreads) words[w] = w < a.words_count ? a.words[w] : 0;
+  }
   for (int i = tid; i < a.n; i += kCompactThreads) bad |= a.lens[i] < 0 || pages_of(a.lens[i], a.page_shift) > a.max_pages;
   const bool bad_lens = __syncthreads_or(bad) != 0;
   int sum = 0;
@@ -493,6 +510,7 @@ __global__ __launch_bounds__(kCompactThreads) void k_compact_apply(CompactArgs a
     *a.move_count = moved;
     *a.status = status;
   }
+  if constexpr (kAlone) return;
   // the last block clears the bitmap: all others have read it
   __syncthreads();
   if (tid == 0) last = atomicAdd(a.arrived, 1) == static_cast<int>(gridDim.x) - 1;
@@ -632,7 +650,7 @@ int soc_paged_fork(soc_ctx* ctx, int32_t n, const int32_t* parents, const int32_
   auto* mark = n <= soc::kSmallThreads ? soc::k_fork_mark<1> : soc::k_fork_mark<4>;
   hipLaunchKernelGGL(mark, dim3(blocks), dim3(soc::kSmallThreads), 0, ctx->stream, a);
   hipLaunchKernelGGL(soc::k_fork_find, dim3(std::min(units, 2048)), dim3(soc::kForkThreads), 0, ctx->stream, a);
-  hipLaunchKernelGGL(soc::k_fork_give, dim3(std::min(units, 256)), dim3(soc::kForkThreads), 0, ctx->stream, a);
+  hipLaunchKernelGGL(soc::k_fork_give, dim3(std::min(units, 1024)), dim3(soc::kForkThreads), 0, ctx->stream, a);
   return soc::hip_status(hipGetLastError(), "paged fork");
   SOC_API_END
 }
@@ -705,9 +723,6 @@ int soc_paged_compact(soc_ctx* ctx, int32_t n, const int32_t* lens, int32_t page
   if ((new_table != block_table && soc::overlap(block_table, span, new_table, span, 4)) ||
       (new_ring != free_ring && soc::overlap(free_ring, num_pages, new_ring, num_pages, 4)))
     return soc::fail(SOC_ERR_INVALID, "paged compact: table and ring are updated in place or have no byte in common");
-  soc::PageWords words;
-  SOC_TRY(soc::ensure_page_words(ctx, num_pages, &words));
-  SOC_TRY(soc::ensure_serve_ws(ctx, 0, 1));
   soc::CompactArgs a{};
   a.n = n;
   a.lens = lens;
@@ -724,19 +739,29 @@ int soc_paged_compact(soc_ctx* ctx, int32_t n, const int32_t* lens, int32_t page
   a.max_moves = max_moves;
   a.move_count = move_count;
   a.status = status;
-  a.words = words.bits;
   a.words_count = (num_pages + 31) / 32;
-  a.arrived = ctx->serve_counters;
   int room = soc::kCompactThreads;
   while (room < a.words_count) room *= 2;
   const size_t lds = static_cast<size_t>(room) * 4;  // at most 128 KiB
+  const int64_t most = std::max<int64_t>(num_pages, static_cast<int64_t>(n) * max_pages);
+  dim3 blocks(static_cast<uint32_t>(std::min<int64_t>(256, (most + soc::kCompactThreads - 1) / soc::kCompactThreads)));
+  // in place, a block could write the ring while another still reads it: there one block does a small pool
+  const bool one = new_ring == free_ring && most <= 16 * soc::kCompactThreads;
+  if (one) blocks.x = 1;
+  if (num_pages <= soc::kAlonePages && (one || new_ring != free_ring)) {
+    hipLaunchKernelGGL(soc::k_compact_apply<true>, blocks, dim3(soc::kCompactThreads), lds, ctx->stream, a);
+    return soc::hip_status(hipGetLastError(), "paged compact");
+  }
+  soc::PageWords words;
+  SOC_TRY(soc::ensure_page_words(ctx, num_pages, &words));
+  SOC_TRY(soc::ensure_serve_ws(ctx, 0, 1));
+  a.words = words.bits;
+  a.arrived = ctx->serve_counters;
   if (lds > (size_t{48} << 10))
-    SOC_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(soc::k_compact_apply),
+    SOC_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(soc::k_compact_apply<false>),
                                     hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
   hipLaunchKernelGGL(soc::k_compact_mark, dim3(std::min(256, (num_pages + 255) / 256)), dim3(256), 0, ctx->stream, a);
-  const int64_t most = std::max<int64_t>(num_pages, static_cast<int64_t>(n) * max_pages);
-  const int blocks = static_cast<int>(std::min<int64_t>(256, (most + soc::kCompactThreads - 1) / soc::kCompactThreads));
-  hipLaunchKernelGGL(soc::k_compact_apply, dim3(blocks), dim3(soc::kCompactThreads), lds, ctx->stream, a);
+  hipLaunchKernelGGL(soc::k_compact_apply<false>, blocks, dim3(soc::kCompactThreads), lds, ctx->stream, a);
   return soc::hip_status(hipGetLastError(), "paged compact");
   SOC_API_END
 }

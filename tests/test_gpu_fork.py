@@ -384,7 +384,7 @@ def check_compact(ctx, lens, page, table, ring, cursors, max_moves, status=0, in
     return want
 
 
-@pytest.mark.parametrize("n,width,spare", [(1, 1, 0), (1, 1, 1), (1, 5, 300), (7, 9, 3), (30, 40, 400), (200, 64, 70000),
+@pytest.mark.parametrize("n,width,spare", [(1, 1, 0), (1, 1, 1), (1, 5, 300), (7, 9, 3), (30, 40, 400), (200, 64, 70000), (9, 9, 300000),
                                            (1000, 20, 5)])
 def test_compact(gpu_ctx, n, width, spare):
     rng = np.random.default_rng(n + spare)
