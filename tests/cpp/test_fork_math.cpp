@@ -1,5 +1,6 @@
-// Index arithmetic of forked rows and of a pool's bitmap (soc_amd/csrc/paged_math.h) against loops that say what it means,
-// with hostile lengths and parents.
+// Index arithmetic of forked rows, of a pool's bitmap and of keys split into chunks (soc_amd/csrc/paged_math.h) against loops
+// that say what it means, with hostile lengths and parents.
+#include <algorithm>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
@@ -67,6 +68,27 @@ int main() {
         }
         for (size_t r = 0; r < free.size(); ++r) CHECK(free_page(f, static_cast<int32_t>(r)) == free[r]);
       }
+  // chunks of any number of keys, also of more than they were laid out for: whole multiples of `least`, all keys in them, none
+  // empty, no more of them than the grid has blocks or a unit has room
+  constexpr int64_t kMostKeys = int64_t{1} << 26;  // of 2^18 pages of 256
+  for (int64_t units : {int64_t{1}, int64_t{3}, int64_t{64}, int64_t{1000}, int64_t{32768}, int64_t{1} << 24})
+    for (int64_t longest : {int64_t{1}, int64_t{31}, int64_t{128}, int64_t{4097}, int64_t{131072}, kMostKeys})
+      for (int32_t waves : {256, 512, 2048})
+        for (int32_t least : {32, 128})
+          for (int32_t most : {128, 256, 1024})
+            for (int32_t room : {1, 16, 64}) {
+              const Chunks c = chunks_for(units, longest, waves, least, most, room);
+              CHECK(c.splits >= 1 && c.splits <= room && c.grid >= 1 && c.grid <= room && c.least == least && c.most == most);
+              for (int64_t keys : {int64_t{0}, int64_t{1}, int64_t{32}, int64_t{33}, int64_t{127}, int64_t{129}, longest - 1, longest,
+                                   4 * longest, kMostKeys}) {
+                if (keys > kMostKeys) continue;
+                const int32_t k = static_cast<int32_t>(keys), chunk = chunk_of(k, c), many = chunks_of(k, chunk);
+                CHECK(chunk > 0 && chunk % least == 0);
+                CHECK(many >= 0 && many <= c.grid && (many == 0) == (k == 0));
+                CHECK(static_cast<int64_t>(many) * chunk >= k && (many == 0 || static_cast<int64_t>(many - 1) * chunk < k));
+                if (k > 0 && c.grid >= ((k - 1) / most / c.splits + 1) * static_cast<int64_t>(c.splits)) CHECK(chunk <= std::max(most, least));
+              }
+            }
   std::printf("fork math ok\n");
   return 0;
 }

@@ -158,3 +158,55 @@ def test_two_contexts_in_turn(gpu_ctx):
             check_fork((other, gpu_ctx)[i % 2], parents, keep, old, 16, table, ring, cursors)
     finally:
         other.close()
+
+
+def test_copies_and_shared_pages_beyond_32_bit_offsets(gpu_ctx, monkeypatch):
+    """A pool of more than 2^32 elements each of keys and values: pages at its end are copied to its front and back, and attended
+    to by a group whose columns fill blocks and by one of a few columns."""
+    monkeypatch.setenv("SOC_PAGED_SHARED", "always")
+    from tests.test_gpu_paged_shared import formula
+
+    ctx, rng = gpu_ctx, np.random.default_rng(6)
+    page, nkv, nq, hd, sizes, prefix, tail = 256, 8, 16, 128, [12, 2], 512, 30
+    per = nkv * page * hd
+    pages, n = (1 << 32) // per + 40, sum(sizes)
+    common = rng.standard_normal((2, 2, 2, nkv, page, hd)).astype(np.float16)  # [group][place][k, v]
+    own = rng.standard_normal((n, 2, nkv, page, hd)).astype(np.float16)
+    q = rng.standard_normal((n, nq * hd)).astype(np.float32)
+    pk, pv = ctx.alloc(pages * per * 2), ctx.alloc(pages * per * 2)
+    # written at the front or at the end, copied to the other: where they are read
+    moves = np.array([[3, pages - 1, page], [pages - 2, 4, page], [5, pages - 3, page], [pages - 4, 6, 200]], np.int32)
+    table = np.zeros((n, 3), np.int32)
+    table[: sizes[0], :2] = [pages - 1, 4]
+    table[sizes[0]:, :2] = [pages - 3, pages - 9]
+    table[:, 2] = np.where(np.arange(n) % 2, np.arange(n) + 10, pages - 10 - np.arange(n))
+    try:
+        with Arrays(ctx) as mem:
+            def write(p, kv):
+                ctx.write(pk + int(p) * per * 2, kv[0])
+                ctx.write(pv + int(p) * per * 2, kv[1])
+
+            for p, kv in ((3, common[0, 0]), (pages - 2, common[0, 1]), (5, common[1, 0]), (pages - 9, common[1, 1])):
+                write(p, kv)
+            for r in range(n):
+                write(table[r, 2], own[r])
+            write(pages - 4, own[0])
+            write(6, own[1])
+            cache = S.PagedCache(pk, pv, pages, page, nkv, hd)
+            S.paged_copy(ctx, S.PagedLayers([cache]), mem.up(moves), None, len(moves))
+            out = mem.up(np.zeros_like(q))
+            S.paged_attention_shared(ctx, cache, mem.up(q), nq * hd, "f32", mem.up(table), 3, 3,
+                                     mem.up(np.full(n, prefix + tail, np.int32)), n, mem.up(np.array([0, 12, 14], np.int32)),
+                                     mem.up(np.full(2, prefix, np.int32)), 2, 12, prefix, nq, 0.0, out, nq * hd)
+            got = mem.down(out).reshape(n, nq, hd)
+            part = ctx.download(pv + 6 * per * 2, (nkv, page, hd), np.float16)
+    finally:
+        ctx.synchronize()
+        ctx.free(pk)
+        ctx.free(pv)
+    assert np.array_equal(part[:, :200], own[0, 1][:, :200]) and np.array_equal(part[:, 200:], own[1, 1][:, 200:])
+    for r in range(n):
+        g = int(r >= sizes[0])
+        k, v = (np.concatenate([common[g, 0, i], common[g, 1, i], own[r, i][:, :tail]], 1) for i in range(2))
+        want, _, tol, _ = formula(q[r].reshape(nq, hd), k, v, 1 / math.sqrt(hd))
+        assert (np.abs(got[r] - want) <= tol).all(), r
