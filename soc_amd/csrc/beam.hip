@@ -16,6 +16,9 @@ namespace soc {
 namespace {
 
 constexpr int kMaxStops = 8;
+// Counters: each has a cache line to itself, where additions take their turns (64 requests of 8 beams, 19 chunks each: 71 us, with
+// neighbouring counters 79).
+constexpr int kApart = 32;
 
 struct BeamRow {  // of a whole row: largest logit and log S; NaN where the row offers nothing
   double log_s;
@@ -32,6 +35,7 @@ struct BeamArgs {
   int top_n;
   int stops[kMaxStops], num_stops;
   int chunks;  // of a row
+  bool at_once;  // the last block of a request joins all chunks of its beams
   int first_row;                 // of the launch
   f32x2* parts;                  // [rows][chunks]: largest logit, sum
   uint64_t* tops;                // [rows][chunks][n]: first tokens in order, 0 where there are fewer
@@ -172,15 +176,23 @@ __device__ __forceinline__ void block_first(const float (&v)[E], float best, boo
 }
 
 // LDS beside the static: a chunk's candidates, or the first n of every chunk and those of them at the threshold; then the
-// scores of every beam's first n, and which of them are at the threshold.
-__host__ __device__ constexpr size_t beam_room(int n, int each, int chunks, int beams) {
-  const size_t row = static_cast<size_t>(n) * (each > 2 * chunks ? each : 2 * chunks) * 8, group = static_cast<size_t>(n) * beams * 12;
+// scores of every beam's first n, and which of them are at the threshold. At once: of every chunk's, and their keys.
+__host__ __device__ constexpr size_t beam_room(int n, int each, int chunks, int beams, bool at_once) {
+  const size_t row = static_cast<size_t>(n) * (at_once || each > 2 * chunks ? each : 2 * chunks) * 8;
+  const size_t group = static_cast<size_t>(n) * beams * (at_once ? chunks * 20 : 12) + 8;
   return row > group ? row : group;
+}
+// Whether a request's chunks are joined at once, or row by row and then its rows. The second join takes 1 us (one request of 4
+// beams, 151936 fp32 logits each, n 8: 12.9 us, at once 12.0), which the block that joins all makes up for where they have
+// many first tokens (16 of 4 fp16 beams, n 12, 912 tokens a request: 19.4 us, at once 19.6). The threshold is sought among 256
+// words, two or more a chunk.
+constexpr bool joined_at_once(int n, int chunks, int beams) {
+  return chunks > 1 && chunks * beams <= 128 && chunks * beams * n <= 768;
 }
 
 // One block per chunk of a row, as in soc_logprobs: 256 threads with E logits each in registers. The last block of a row to
-// finish joins its chunks, the last of a request its beams.
-template <typename T, int E>
+// finish joins its chunks, the last of a request its beams; or that does both.
+template <typename T, int E, bool kAtOnce>
 __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k_beam(BeamArgs a) {
   constexpr int VW = 16 / sizeof(T), NV = E / VW, C = kThreads * E;
   typedef T Vec __attribute__((ext_vector_type(VW), aligned(sizeof(T))));
@@ -191,6 +203,8 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   __shared__ uint64_t threshold;
   __shared__ int giver[kMaxTop];
   __shared__ int found, givers, flag, tied;
+  __shared__ double row_log_s[kMaxTop];
+  __shared__ float row_most[kMaxTop];
 
   const int64_t r = blockIdx.x / a.chunks;  // of the launch
   const int c = blockIdx.x % a.chunks, n = a.n;
@@ -244,19 +258,25 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   __syncthreads();
 
   double s = part;
-  if (a.chunks > 1) {
-    f32x2* parts = a.parts + r * a.chunks;
-    uint64_t* tops = a.tops + r * a.chunks * n;
-    if (tid == 0) st_agent(reinterpret_cast<uint64_t*>(parts + c), __builtin_bit_cast(uint64_t, f32x2{m, part}));
-    if (tid < n) st_agent(tops + c * n + tid, first[tid]);
-    if (!arrives_last(a.row_arrived + r, a.chunks, &flag)) return;
-    // every wave the same sums, lane l chunk l (at most 64)
+  // the wave's m and s of a whole row: lane l chunk l (at most 64)
+  const auto whole = [&](int64_t row) {
     f32x2 mine = f32x2{-INFINITY, 0.0f};
-    if (lane < a.chunks) mine = __builtin_bit_cast(f32x2, ld_agent(reinterpret_cast<const uint64_t*>(parts + lane)));
-    for (int i = tid; i < a.chunks * n; i += kThreads) keys[i] = ld_agent(tops + i);
+    if (lane < a.chunks)
+      mine = __builtin_bit_cast(f32x2, ld_agent(reinterpret_cast<const uint64_t*>(a.parts + row * a.chunks + lane)));
     m = wave_max(mine[0]);
     const double from = m == -INFINITY ? 0.0 : static_cast<double>(m);
     s = wave_sum(mine[1] * exp2((mine[0] - from) * (a.inv_t * 1.4426950408889634074)));
+  };
+  if (a.chunks > 1) {
+    uint64_t* tops = a.tops + r * a.chunks * n;
+    if (tid == 0) st_agent(reinterpret_cast<uint64_t*>(a.parts + r * a.chunks + c), __builtin_bit_cast(uint64_t, f32x2{m, part}));
+    if (tid < n) st_agent(tops + c * n + tid, first[tid]);
+  }
+  if (!kAtOnce && a.chunks > 1) {
+    const uint64_t* tops = a.tops + r * a.chunks * n;
+    if (!arrives_last(a.row_arrived + r * kApart, a.chunks, &flag)) return;
+    for (int i = tid; i < a.chunks * n; i += kThreads) keys[i] = ld_agent(tops + i);
+    whole(r);  // by every wave
     // the first few of each chunk give a threshold that at least n of all keys reach, and seldom many more
     const int all = a.chunks * n, few = min(n, (n - 1) / a.chunks + 2);
     uint64_t* left = keys + all;
@@ -280,25 +300,43 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
 
   // the row, then the request's beams
   const int64_t g = r / a.beams;
-  const double log_s = s > 0.0 ? log(s) : __builtin_nan("");  // nothing but -inf, or a NaN or +inf among the logits
-  if (tid < n) st_agent(a.row_tops + r * n + tid, first[tid]);
-  if (tid == 0) {
-    st_agent(reinterpret_cast<uint64_t*>(&a.rows[r].log_s), __builtin_bit_cast(uint64_t, log_s));
-    st_dev(&a.rows[r].m, m);
+  const auto log_of = [](double sum) {  // NaN: nothing but -inf, or a NaN or +inf among the logits
+    return sum > 0.0 ? log(sum) : __builtin_nan("");
+  };
+  if (!kAtOnce) {
+    if (tid < n) st_agent(a.row_tops + r * n + tid, first[tid]);
+    if (tid == 0) {
+      st_agent(reinterpret_cast<uint64_t*>(&a.rows[r].log_s), __builtin_bit_cast(uint64_t, log_of(s)));
+      st_dev(&a.rows[r].m, m);
+    }
   }
-  if (!arrives_last(a.group_arrived + g, a.beams, &flag)) return;
-  const int all = a.beams * n;
+  const int lists = kAtOnce ? a.beams * a.chunks : a.beams, all = lists * n, per = all / a.beams;
+  if (!arrives_last(a.group_arrived + g * kApart, lists, &flag)) return;
   const int row0 = static_cast<int>(g) * a.beams;  // of the launch
-  const uint64_t* row_tops = a.row_tops + static_cast<int64_t>(row0) * n;
+  const uint64_t* tops = (kAtOnce ? a.tops : a.row_tops) + static_cast<int64_t>(row0) * per;
   uint64_t* scores = keys;
   int* left = reinterpret_cast<int*>(keys + all);
+  uint64_t* kept = keys + all + (all + 1) / 2;  // at once: the keys
   if (tid == 0) found = 0;
+  if (kAtOnce) {
+    for (int i = tid; i < all; i += kThreads) kept[i] = ld_agent(tops + i);
+    for (int b = wid; b < a.beams; b += kThreads / kWave) {
+      whole(row0 + b);
+      if (lane == 0) {
+        row_log_s[b] = log_of(s);
+        row_most[b] = m;
+      }
+    }
+    __syncthreads();
+  }
+  const auto key_of_place = [&](int i) { return kAtOnce ? kept[i] : ld_agent(tops + i); };
   for (int i = tid; i < all; i += kThreads) {
-    const int b = i / n;
-    const uint64_t key = ld_agent(row_tops + i);
+    const int b = i / per;
+    const uint64_t key = key_of_place(i);
     const BeamRow* row = a.rows + row0 + b;
-    const double log_sum = __builtin_bit_cast(double, ld_agent(reinterpret_cast<const uint64_t*>(&row->log_s)));
-    const float most = ld_dev(&row->m), cum = a.scores[a.first_row + row0 + b];
+    const double log_sum = kAtOnce ? row_log_s[b]
+                                   : __builtin_bit_cast(double, ld_agent(reinterpret_cast<const uint64_t*>(&row->log_s)));
+    const float most = kAtOnce ? row_most[b] : ld_dev(&row->m), cum = a.scores[a.first_row + row0 + b];
     const float logit = value_of<T>(static_cast<uint32_t>(key >> 32));
     const double score = (static_cast<double>(logit) - most) * a.inv_t - log_sum + cum;
     // no token; a masked one; a beam that is none or whose row offers nothing
@@ -309,13 +347,13 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   // candidates: all, or where they are many those at a threshold that at least n reach
   uint32_t t = 1;
   if (all > kThreads) {
-    const int few = min(n, (n - 1) / a.beams + 2);  // at most 64 + 2 * 64 words
+    const int few = min(n, (n - 1) / lists + 2);  // at most 256 words
     if (wid == 0) {
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = j * kWave + lane;
-        w[j] = i < a.beams * few ? static_cast<uint32_t>(scores[i / few * n + i % few] >> 32) : 0;
+        w[j] = i < lists * few ? static_cast<uint32_t>(scores[i / few * n + i % few] >> 32) : 0;
       }
       bool exact;
       const uint32_t o = nth_word(w, n, 0, &exact);
@@ -331,12 +369,18 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   for (int k = tid; k < many; k += kThreads) {
     const int i = left[k];
     const uint64_t score = scores[i];
-    int rank = 0;
+    int rank = 0, same = 0;
+#pragma unroll 4
     for (int u = 0; u < many; ++u) {
-      const int j = left[u];
-      const uint64_t other = scores[j];
-      rank += other > score || (other == score && j < i);
+      const uint64_t other = scores[left[u]];
+      rank += other > score;
+      same += other == score;
     }
+    if (same > 1)  // the first beam's, then the larger logit's or the first token's
+      for (int u = 0; u < many; ++u) {
+        const int j = left[u];
+        if (scores[j] == score) rank += kAtOnce && j / per == i / per ? kept[j] > kept[i] : j < i;
+      }
     if (rank < n) group[rank] = i;
   }
   __syncthreads();
@@ -345,8 +389,8 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
   float score = -INFINITY;
   if (lane < n && group[lane] != ~uint64_t{0}) {
     const int i = static_cast<int>(group[lane]);
-    row = a.first_row + row0 + i / n;
-    token = kMaxVocab - static_cast<int32_t>(static_cast<uint32_t>(ld_agent(row_tops + i)));
+    row = a.first_row + row0 + i / per;
+    token = kMaxVocab - static_cast<int32_t>(static_cast<uint32_t>(key_of_place(i)));
     score = static_cast<float>(score_value(scores[i]));
   }
   const int64_t request = a.first_row / a.beams + g;
@@ -374,8 +418,8 @@ __global__ __launch_bounds__(kThreads, E == 32 && sizeof(T) == 4 ? 8 : 4) void k
 
 template <typename T, int E>
 hipError_t launch_beam(const BeamArgs& a, int rows, hipStream_t s) {
-  hipLaunchKernelGGL((k_beam<T, E>), dim3(static_cast<uint32_t>(rows) * a.chunks), dim3(kThreads),
-                     beam_room(a.n, E, a.chunks, a.beams), s, a);
+  hipLaunchKernelGGL((a.at_once ? k_beam<T, E, true> : k_beam<T, E, false>), dim3(static_cast<uint32_t>(rows) * a.chunks),
+                     dim3(kThreads), beam_room(a.n, E, a.chunks, a.beams, a.at_once), s, a);
   return hipGetLastError();
 }
 template <typename T>
@@ -431,13 +475,14 @@ int soc_beam_select(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row
   soc::BeamArgs a{};
   a.chunks = chunks_of(each);
   a.n = next ? std::max(top_n, beams * (1 + num_stops)) : top_n;
+  a.at_once = soc::joined_at_once(a.n, a.chunks, beams);
   // groups a launch: its workspace stays below 32 MiB (or is one group's), its work-items below 2^32
   const size_t per_row = a.chunks * (8 + static_cast<size_t>(a.n) * 8) + sizeof(soc::BeamRow) + static_cast<size_t>(a.n) * 8;
   const int64_t most = std::min<int64_t>((int64_t{32} << 20) / static_cast<int64_t>(per_row * beams),
                                          (int64_t{1} << 23) / (static_cast<int64_t>(a.chunks) * beams));
   const int step = static_cast<int>(std::min<int64_t>(groups, std::max<int64_t>(1, most)));
   const size_t step_rows = static_cast<size_t>(step) * beams;
-  SOC_TRY(soc::ensure_serve_ws(ctx, step_rows * per_row, step_rows + step));
+  SOC_TRY(soc::ensure_serve_ws(ctx, step_rows * per_row, (step_rows + step) * soc::kApart));
   a.row_stride = row_stride;
   a.logits = logits;
   a.beams = beams;
@@ -454,7 +499,7 @@ int soc_beam_select(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row
   a.rows = reinterpret_cast<soc::BeamRow*>(a.row_tops + step_rows * a.n);
   a.parts = reinterpret_cast<soc::f32x2*>(a.rows + step_rows);
   a.row_arrived = ctx->serve_counters;
-  a.group_arrived = ctx->serve_counters + step_rows;
+  a.group_arrived = ctx->serve_counters + step_rows * soc::kApart;
   a.top_rows = top_rows;
   a.top_tokens = top_tokens;
   a.top_scores = top_scores;
