@@ -238,3 +238,19 @@ def test_beam_refuses(gpu_ctx):
             assert e.value.code == SOC_ERR_INVALID
         call()
         gpu_ctx.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("beams,top", [(2, 6), (4, 8), (4, 40), (9, 18)])
+def test_beam_of_equal_scores(gpu_ctx, dtype, beams, top):
+    """A temperature at which all tokens are equally likely: a beam's come by logit, whichever part of the row they lie in."""
+    rng = np.random.default_rng(top)
+    x = rng.normal(0, 1, (2 * beams, 30001))
+    check(gpu_ctx, x, dtype, np.full(2 * beams, -1.5), 2, beams, 2.0 ** 100, [], top, exact=True)
+
+
+@pytest.mark.parametrize("beams,top", [(1, 64), (2, 6), (4, 64), (64, 64)])
+def test_beam_of_the_largest_vocabulary(gpu_ctx, beams, top):
+    rng = np.random.default_rng(beams)
+    x = rng.standard_normal((beams, 1 << 20), np.float32) * np.float32(2.5)
+    check(gpu_ctx, x, "f16", -5 * rng.random(beams), 1, beams, 1.0, [], top)
