@@ -484,7 +484,8 @@ int soc_paged_copy(soc_ctx* ctx, const soc_paged_cache* caches, int32_t layers, 
  * lowest free page, for as long as that is a lower one, at most max_moves times. moves [max_moves][3], of which *move_count
  * are written: (from, to, page_size), as soc_paged_copy takes them, which has to follow before the cache is used.
  * new_table: the n rows' entries within lens, moved pages by their new ids (entries behind them left as they are). new_ring:
- * the free pages at the same places head .. tail - 1, lowest first; the cursors hold on. With enough moves the first
+ * the free pages at the same places head .. tail - 1, lowest first; the cursors hold on. What else names pages of the pool
+ * has to follow the moves. With enough moves the first
  * num_pages - (tail - head) pages are those in use. new_table may be block_table, new_ring free_ring; else they must not
  * overlap. num_pages <= 2^20. *status = 0; or bits, and then nothing moves: SOC_PLAN_LENGTHS, a length out of range;
  * SOC_PLAN_CURSORS, cursors out of range, or free entries that are no page of the pool or the same one twice. */
@@ -500,7 +501,8 @@ int soc_paged_compact(soc_ctx* ctx, int32_t n, const int32_t* lens, int32_t page
  * caller's word. For the rest the groups are a hint: starts that do not ascend within the n rows, prefixes that are negative,
  * longer than a row or than max_prefix, rows beyond max_group in a group, prefixes too short to be worth it: then a row's
  * keys are read from its own pages. 1 <= groups <= 4096, no more than n. max_group (at least 1) and max_prefix (at least 0)
- * bound what is launched.
+ * bound what is launched. Small batches, and those without a group of two or a prefix worth it, are answered by
+ * soc_paged_attention_decode itself.
  * Everything else as there; a row's bits follow also from its group's size and prefix and from its place in it, not from
  * the other rows' lengths or contents. A page outside the cache within the prefix makes all rows that read it NaN. */
 int soc_paged_attention_shared(soc_ctx* ctx, const soc_paged_cache* cache, const void* q, int64_t q_stride, int32_t dtype,

@@ -18,7 +18,10 @@
 // The reference follows a score only where that gives a weight above 2^14, and then makes it 2^10: the sums are seldom
 // rescaled, and no maximum is sought otherwise. l is another row of O^T, of values 1.
 //
-// FIGURES
+// Bound: reading keys and values once. 256 rows behind 4096 common keys with 512 of their own, 32 query and 8 KV heads of 128,
+// fp32: 136 us, of which 131 reading 589 MB (4.4 TB/s; a large copy reaches 4.7); read row by row they would be 4.8 GB.
+// 24 groups of ragged rows in fp16, 259 MB: 66.7 us, 4.4 TB/s and 6 us of joining. The products of a prefix take 8.7 us per 1000
+// keys of those 256 rows, 0.97 PFLOP/s with both parts (a large fp16 product reaches 1.2): more than its reading beyond 64 rows.
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>

@@ -142,9 +142,9 @@ def some_parents(rng, n, old):
     return parents, keep
 
 
-# rows x width: one block (up to 16384 entries) and three launches, chunks of 256 columns, 256 / 1024 / 4096 rows
+# rows x width: one block (up to 2048 entries) and three launches, chunks of 256 columns, 256 / 1024 / 4096 rows
 @pytest.mark.parametrize("n,width,page", [
-    (1, 1, 16), (1, 70, 16), (2, 3, 256), (4, 63, 16), (16, 100, 32), (64, 256, 16), (1000, 16, 64), (1024, 16, 16),
+    (1, 1, 16), (1, 70, 16), (2, 3, 256), (4, 63, 16), (16, 100, 32), (1000, 2, 16), (8, 255, 32), (64, 256, 16), (1000, 16, 64), (1024, 16, 16),
     (65, 256, 16), (1025, 3, 16), (4096, 4, 16), (4096, 5, 128), (3, 9000, 16), (20, 1030, 32), (300, 70, 16), (700, 513, 16)])
 def test_fork_mixed(gpu_ctx, n, width, page):
     rng = np.random.default_rng(n * 31 + width)
@@ -167,7 +167,7 @@ def test_fork_mixed(gpu_ctx, n, width, page):
     ([0, 0, 0, 0], [64, 64, 64, 64], [64, 64, 64, 64])])
 def test_fork_edges(gpu_ctx, parents, keep, old, small):
     rng = np.random.default_rng(3)
-    width = 4 if small else 16000  # beyond 16384 entries
+    width = 4 if small else 16000  # beyond what one block takes
     n = len(old)
     if not small and n == 1:
         width = 17000
