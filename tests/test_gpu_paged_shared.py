@@ -156,7 +156,7 @@ def ragged(rng, sizes, longest):
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("hd,page", [(128, 16), (64, 32), (128, 64), (64, 256), (128, 128)])
 @pytest.mark.parametrize("sizes,prefix", [([4], [1000]), ([2, 3, 1], [128, 400, 300]), ([1, 1], [200, 150]), ([8], [127]),
-                                          ([9, 2], [1025, 31]), ([3, 5], [0, 2311])])
+                                          ([9, 2], [1025, 31]), ([3, 5], [0, 2311]), ([8, 3], [255, 256]), ([3, 7], [288, 257])])
 def test_groups(gpu_ctx, dtype, hd, page, sizes, prefix):
     rng = np.random.default_rng(page + hd)
     b = Batch(sizes, prefix, ragged(rng, sizes, 150), 8, 2, hd, page)
