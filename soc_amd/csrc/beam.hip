@@ -477,7 +477,8 @@ int soc_beam_select(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row
   a.n = next ? std::max(top_n, beams * (1 + num_stops)) : top_n;
   a.at_once = soc::joined_at_once(a.n, a.chunks, beams);
   // groups a launch: its workspace stays below 32 MiB (or is one group's), its work-items below 2^32
-  const size_t per_row = a.chunks * (8 + static_cast<size_t>(a.n) * 8) + sizeof(soc::BeamRow) + static_cast<size_t>(a.n) * 8;
+  const size_t per_row = a.chunks * (8 + static_cast<size_t>(a.n) * 8) + sizeof(soc::BeamRow) + static_cast<size_t>(a.n) * 8 +
+                         2 * soc::kApart * sizeof(int);
   const int64_t most = std::min<int64_t>((int64_t{32} << 20) / static_cast<int64_t>(per_row * beams),
                                          (int64_t{1} << 23) / (static_cast<int64_t>(a.chunks) * beams));
   const int step = static_cast<int>(std::min<int64_t>(groups, std::max<int64_t>(1, most)));

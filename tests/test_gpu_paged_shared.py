@@ -354,3 +354,23 @@ def test_refusals(gpu_ctx):
             assert e.value.code == SOC_ERR_INVALID, kw
         call()
         gpu_ctx.synchronize()
+
+
+def test_refuses_bounds_beyond_a_launch(gpu_ctx):
+    n, nkv, nq, hd, page = 4096, 2, 32, 64, 16
+    with Arrays(gpu_ctx) as mem:
+        pool = np.zeros((20, nkv, page, hd), np.float16)
+        cache = S.PagedCache(mem.up(pool), mem.up(pool), 20, page, nkv, hd)
+        q, out = (mem.up(np.zeros((n, nq * hd), np.float32)) for _ in range(2))
+        t, lens, prefix = mem.up(np.zeros((n, 256), np.int32)), mem.up(np.zeros(n, np.int32)), mem.up(np.zeros(n, np.int32))
+        starts = mem.up(np.arange(n + 1, dtype=np.int32))
+
+        def call(max_group):
+            S.paged_attention_shared(gpu_ctx, cache, q, nq * hd, "f32", t, 256, 256, lens, n, starts, prefix, n, max_group, 4096,
+                                     nq, 0.0, out, nq * hd)
+
+        with pytest.raises(S.SocError, match="too many groups") as e:
+            call(n)
+        assert e.value.code == SOC_ERR_INVALID
+        call(2)
+        assert not mem.down(out).any()
