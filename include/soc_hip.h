@@ -502,8 +502,8 @@ int soc_paged_compact(soc_ctx* ctx, int32_t n, const int32_t* lens, int32_t page
  * longer than a row or than max_prefix, rows beyond max_group in a group, prefixes too short to be worth it: then a row's
  * keys are read from its own pages. 1 <= groups <= 4096, no more than n. max_group (at least 1) and max_prefix (at least 0)
  * bound what is launched; bounds that ask for more than 2^23 blocks (a block: 64 columns of max_group * q_heads / kv_heads
- * of a group and KV head, up to 1024 keys of max_prefix) are refused. Small batches, and those without a group of two or a prefix worth it, are answered by
- * soc_paged_attention_decode itself.
+ * of a group and KV head, up to 1024 keys of max_prefix) are refused. Small batches, and those without a group of two or a
+ * prefix worth it, are answered by soc_paged_attention_decode itself.
  * Everything else as there; a row's bits follow also from its group's size and prefix and from its place in it, not from
  * the other rows' lengths or contents. A page outside the cache within the prefix makes all rows that read it NaN. */
 int soc_paged_attention_shared(soc_ctx* ctx, const soc_paged_cache* cache, const void* q, int64_t q_stride, int32_t dtype,

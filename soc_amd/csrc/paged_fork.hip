@@ -15,10 +15,9 @@ namespace {
 // Whether a page is still named is found from the tables alone: no counts are kept that could go wrong. Each page has a
 // 64-bit word that outlives the call; its upper 48 bits are the call that wrote it last, so that nothing is cleared. Every
 // entry of the new table (but where the row before has the same page, which is then marked already) raises its page's word to
-// (call, all ones); every entry that a row loses (its old page at a place
-// where its new one is another, or none) raises it to (call, row + 1). Afterwards (call, row + 1) stands exactly at the pages
-// that no row names any more, with the last row that lost them; that row's entry puts the page into the ring. Maxima do not
-// depend on order.
+// (call, all ones); every entry that a row loses (its old page at a place where its new one is another, or none) raises it to
+// (call, row + 1). Afterwards (call, row + 1) stands exactly at the pages that no row names any more, with the last row that
+// lost them; that row's entry puts the page into the ring. Maxima do not depend on order.
 struct ForkArgs {
   int n;
   const int32_t *parents, *keep, *old_lens;

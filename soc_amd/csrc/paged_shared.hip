@@ -20,7 +20,7 @@
 // rescaled, and no maximum is sought otherwise. l is another row of O^T, of values 1.
 //
 // Bound: reading keys and values once. 256 rows behind 4096 common keys with 512 of their own, 32 query and 8 KV heads of 128,
-// fp32: 136 us, of which 131 reading 589 MB (4.4 TB/s; a large copy reaches 4.7); read row by row they would be 4.8 GB.
+// fp32: 130 us, of which 122 reading 589 MB (4.8 TB/s; a large copy reaches 4.7); read row by row they would be 4.8 GB.
 // 24 groups of ragged rows in fp16, 259 MB: 66.7 us, 4.4 TB/s and 6 us of joining. The products of a prefix take 8.7 us per 1000
 // keys of those 256 rows, 0.97 PFLOP/s with both parts (a large fp16 product reaches 1.2): more than its reading beyond 64 rows.
 #include <algorithm>
@@ -207,7 +207,8 @@ __device__ __forceinline__ f16x8 all_ones() {
   return v;
 }
 
-// One wave of four, 16 columns, every fourth tile; kOnce: keys that nobody else reads. Keys and values go from memory to registers, 16 bytes a lane, the next tile's on their way; of
+// One wave of four, 16 columns, every fourth tile; kOnce: keys that nobody else reads, past the caches (256 rows behind 4096
+// common keys 139 us, else 142). Keys and values go from memory to registers, 16 bytes a lane, the next tile's on their way; of
 // the 8 dims x 8 keys of values that a lane reads, v_perm_b32 makes the operand V^T, in whose rows dim d * 16 + i stands for
 // dim i * (HD / 16) + d. Whether a page was none of the cache.
 template <typename T, int HD, bool kOnce>
@@ -558,8 +559,11 @@ __device__ __forceinline__ void prefix_part(const SharedArgs& a, int unit, char*
     const int c = wid * 16 + (lane & 15), at = cols.first + c, r = at / G, h = at - r * G, row = lane >> 4;
     if (c >= cols.count || !holds(r)) return;
     float* part = part_of(r);
+    // past the caches, where the many parts of a block would push out what others read (256 rows behind 4096 common keys 130 us,
+    // with plain stores 138; the parts of the other way, fewer, gain nothing so)
 #pragma unroll
-    for (int d = 0; d < HD / 16; ++d) *reinterpret_cast<Four*>(part + h * HD + d * 16 + row * 4) = sums.o[d];
+    for (int d = 0; d < HD / 16; ++d)
+      __builtin_nontemporal_store(static_cast<Four>(sums.o[d]), reinterpret_cast<Four*>(part + h * HD + d * 16 + row * 4));
     if (row == 0) {
       part[G * HD + h] = sums.m;
       part[G * HD + G + h] = lost ? nan : sums.l[0];
