@@ -156,24 +156,30 @@ __device__ __forceinline__ void clear(Sums<HD>& s) {
 
 // The weights of a tile's scores as P^T operands, high and low parts; the reference moved and the sums rescaled where need
 // be. Of a tile that `left` < 32 keys are in, the others (which repeat the last key) get weight 0.
+// Scores are rounded before the reference is taken from them, as it was rounded itself: it then lies within a rounding of the
+// scores' greatest, however large they are. (The exact product less the reference leaves what the reference was rounded by,
+// which passes the range of a weight for scores from 2^28 on.)
 template <int HD>
 __device__ __forceinline__ void weigh(const f32x4 (&sc)[2], float to_log2, uint32_t left, Sums<HD>& s, f16x8& high,
                                       f16x8& low) {
-  float p[8];
+#pragma clang fp contract(off)
+  float t[8], p[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t[j] = sc[j >> 2][j & 3] * to_log2;
   auto weights = [&] {
     float most = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(fmaf(sc[j >> 2][j & 3], to_log2, -s.m));
+      p[j] = __builtin_amdgcn_exp2f(t[j] - s.m);
       most = fmaxf(most, p[j]);
     }
     return most;
   };
   if (__ballot(!(weights() <= kMostWeight)) != 0) {
-    float top = sc[0][0];
+    float top = t[0];
 #pragma unroll
-    for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[j >> 2][j & 3]);
-    top = across_rows(top, [](float x, float y) { return fmaxf(x, y); }) * to_log2;
+    for (int j = 1; j < 8; ++j) top = fmaxf(top, t[j]);
+    top = across_rows(top, [](float x, float y) { return fmaxf(x, y); });
     const bool moves = !(top - kMostBits <= s.m) && top > -INFINITY;
     const float to = moves ? top - kStartBits : s.m, f = moves ? __builtin_amdgcn_exp2f(s.m - to) : 1.0f;
     s.m = to;

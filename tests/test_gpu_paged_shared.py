@@ -374,3 +374,32 @@ def test_refuses_bounds_beyond_a_launch(gpu_ctx):
         assert e.value.code == SOC_ERR_INVALID
         call(2)
         assert not mem.down(out).any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bits", [10, 24, 28, 33, 40, 64, 100, -28, -64])
+def test_scores_that_fp32_holds_but_not_to_a_unit(gpu_ctx, bits, hd, dtype):
+    """Whole products, times +- 2^|bits|: what a score is off by in 32 bits passes the range of an exponential, but the largest
+    scores are equal ones, and the others' weights are 0 from 2^10 on (e^-1024). So the result is the mean of the values at the
+    largest product, off by their weights' 2^-22 and the chains of additions; lse is that score but for eight roundings (log2(e),
+    ln 2 and the scale's product with it, the score, the reference, its logarithm's sum, the product with ln 2), 2^-21, and the
+    logarithm of their count."""
+    b = Batch([5, 2], [300, 290], [4, 0, 20, 33, 1, 100, 3], 16, 2, hd, 16,
+              kv=lambda row, own: np.stack([np.clip(np.rint(own[0]), -3, 3), own[1]]))
+    b.q[:] = np.clip(np.rint(b.q), -3, 3)
+    scale = math.copysign(2.0 ** abs(bits), bits)
+    out, lse, q = b.run(gpu_ctx, dtype, scale=scale)
+    for r in range(b.n):
+        k, v = b.rows[r].astype(np.float64)
+        s = q[r].astype(np.float64).reshape(2, 8, hd) @ k.transpose(0, 2, 1) * scale
+        top = s.max(-1, keepdims=True)
+        w = (s == top) / (s == top).sum(-1, keepdims=True)
+        want = (w @ v).reshape(16, hd)
+        c = 2 * (2048 // 4 + 32) + 264
+        tol = ((c + 8) * 2.0 ** -24 + 2.0 ** -21) * np.abs(v).max()
+        if dtype == "f16":
+            tol = tol + np.abs(want) * 2.0 ** -11 + 2.0 ** -25
+        assert (np.abs(out[r] - want) <= tol).all(), (r, float(np.abs(out[r] - want).max()))
+        want_lse = (top[..., 0] + np.log((s == top).sum(-1))).reshape(16)
+        assert (np.abs(lse[r] - want_lse) <= 2.0 ** -21 * np.abs(want_lse) + (c + 8) * 2.0 ** -24).all(), (r, lse[r], want_lse)
