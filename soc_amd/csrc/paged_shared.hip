@@ -69,7 +69,7 @@ struct SharedArgs {
 };
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kMostBits = 14.0f, kMostWeight = 16384.0f, kStartBits = 10.0f;
+constexpr float kMostWeight = 16384.0f, kStartBits = 10.0f;
 
 // Reduces over the four lanes l % 16 + {0, 16, 32, 48}; every lane gets the result.
 template <typename F>
@@ -167,20 +167,23 @@ __device__ __forceinline__ void weigh(const f32x4 (&sc)[2], float to_log2, uint3
 #pragma unroll
   for (int j = 0; j < 8; ++j) t[j] = sc[j >> 2][j & 3] * to_log2;
   auto weights = [&] {
-    float most = 0.0f;
+    float largest = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       p[j] = __builtin_amdgcn_exp2f(t[j] - s.m);
-      most = fmaxf(most, p[j]);
+      largest = fmaxf(largest, p[j]);
     }
-    return most;
+    return largest;
   };
-  if (__ballot(!(weights() <= kMostWeight)) != 0) {
+  const float most = weights();
+  if (__ballot(!(most <= kMostWeight)) != 0) {
+    // a column moves by its own weights, whichever other column (of another row, as a rule) brought the wave here
+    const auto larger = [](float x, float y) { return fmaxf(x, y); };
     float top = t[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) top = fmaxf(top, t[j]);
-    top = across_rows(top, [](float x, float y) { return fmaxf(x, y); });
-    const bool moves = !(top - kMostBits <= s.m) && top > -INFINITY;
+    top = across_rows(top, larger);
+    const bool moves = across_rows(most, larger) > kMostWeight && top > -INFINITY;
     const float to = moves ? top - kStartBits : s.m, f = moves ? __builtin_amdgcn_exp2f(s.m - to) : 1.0f;
     s.m = to;
 #pragma unroll

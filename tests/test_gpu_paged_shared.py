@@ -403,3 +403,36 @@ def test_scores_that_fp32_holds_but_not_to_a_unit(gpu_ctx, bits, hd, dtype):
         assert (np.abs(out[r] - want) <= tol).all(), (r, float(np.abs(out[r] - want).max()))
         want_lse = (top[..., 0] + np.log((s == top).sum(-1))).reshape(16)
         assert (np.abs(lse[r] - want_lse) <= 2.0 ** -21 * np.abs(want_lse) + (c + 8) * 2.0 ** -24).all(), (r, lse[r], want_lse)
+
+
+def unit_scale():
+    """A scale whose fp32 product with log2(e) is 1: scores in base 2 are the products themselves."""
+    log2e, s = np.float32(1.4426950408889634), np.float32(math.log(2))
+    for c in [s, *(np.nextafter(s, np.float32(d), dtype=np.float32) for d in (0, 1))]:
+        if np.float32(c * log2e) == 1:
+            return float(c)
+    raise AssertionError("no such scale")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows,nkv,prefix,second", [(3, 1, 256, 32), (2, 256, 1024, 128)])
+def test_a_row_s_bits_at_the_edge_of_a_rescale(gpu_ctx, rows, nkv, prefix, second, dtype):
+    """Row 0's second score lies half a unit in the last place of 14 above its reference and 14: no weight passes 2^14, but the
+    score less 14, rounded, passes the reference. Whether row 1, whose columns the same wave holds, is rescaled at that tile must not
+    show in row 0. Blocks of 64 columns (24 of them, a wave's next tile 32 keys on) and of 16 (128 keys on)."""
+    hd, G = 64, 8
+
+    def kv(row, own):
+        own = own.copy()
+        own[0] = 0
+        own[0, :, 0, :2] = 0.5, 2.0 ** -10            # row 0: 0.5 + 2^-20, reference 2^-20 - 9.5
+        own[0, :, second, :3] = 4.5, 3 * 2.0 ** -11, 100  # row 0: 4.5 + 3 2^-21 = reference + 14 + 2^-21
+        return own
+
+    b = Batch([rows], [prefix], [0] * rows, G * nkv, nkv, hd, 16, kv=kv)
+    q = np.zeros((rows, nkv * G, hd), np.float32)
+    q[0, :, :2] = 1, 2.0 ** -10
+    one = b.run(gpu_ctx, dtype, q=q.reshape(rows, -1), scale=unit_scale())
+    q[1:, :, 2] = 1
+    two = b.run(gpu_ctx, dtype, q=q.reshape(rows, -1), scale=unit_scale())
+    assert np.array_equal(one[0][0], two[0][0]) and np.array_equal(one[1][0], two[1][0])
