@@ -16,8 +16,11 @@ namespace {
 // 64-bit word that outlives the call; its upper 48 bits are the call that wrote it last, so that nothing is cleared. Every
 // entry of the new table (but where the row before has the same page, which is then marked already) raises its page's word to
 // (call, all ones); every entry that a row loses (its old page at a place where its new one is another, or none) raises it to
-// (call, row + 1). Afterwards (call, row + 1) stands exactly at the pages that no row names any more, with the last row that
-// lost them; that row's entry puts the page into the ring. Maxima do not depend on order.
+// its own mark, later rows' above earlier ones'. Afterwards the mark of the last entry that lost it stands exactly at a page that no
+// row names any more; that entry puts the page into the ring. Maxima do not depend on order. One block's tables have so few entries
+// that a mark is (call, the entry's number + 1). In larger ones it is (call, row + 1, 0); an entry that finds its own mark there
+// already, as only in a table that names a page twice in a row, sets the lowest bit, and the entries of such a page look in their row
+// for a later one.
 struct ForkArgs {
   int n;
   const int32_t *parents, *keep, *old_lens;
@@ -167,10 +170,10 @@ __device__ __forceinline__ ForkEntry fork_entry(const ForkArgs& a, const Rows& s
   return e;
 }
 
-// Writes the entry and marks its pages; whether the row lost one.
+// Writes the entry and marks its pages, a lost one with `mark`; whether the row lost one, whose word was *before.
 template <typename Rows>
-__device__ __forceinline__ bool fork_mark(const ForkArgs& a, const Rows& s, int i, int j, const ForkEntry& e,
-                                          uint64_t call) {
+__device__ __forceinline__ bool fork_mark(const ForkArgs& a, const Rows& s, int i, int j, const ForkEntry& e, uint64_t call,
+                                          uint64_t mark, uint64_t* before) {
   if (j < s.pages[i]) {
     a.new_table[i * a.table_stride + j] = e.is;
     if (call != 0 && !e.marked && checked_page(e.is, a.num_pages) >= 0)
@@ -180,18 +183,17 @@ __device__ __forceinline__ bool fork_mark(const ForkArgs& a, const Rows& s, int 
   const bool lost = call != 0 && j < s.held[i] && (j >= s.pages[i] || e.was != e.is) &&
                     checked_page(e.was, a.num_pages) >= 0;
   if (lost)
-    atomicMax(reinterpret_cast<unsigned long long*>(a.marks + e.was),
-              static_cast<unsigned long long>(call << 16 | static_cast<uint32_t>(i + 1)));
+    *before = atomicMax(reinterpret_cast<unsigned long long*>(a.marks + e.was), static_cast<unsigned long long>(mark));
   return lost;
 }
-// Whether row i's entry is the last to have lost its page, which no row names now. After all marks.
+// Whether row i's entry, of mark `mark`, is the last to have lost its page, which no row names now. After all marks.
 template <typename Rows>
 __device__ __forceinline__ bool fork_frees(const ForkArgs& a, const Rows& s, int i, int j, const ForkEntry& e,
-                                           uint64_t call) {
+                                           uint64_t mark) {
   if (j >= s.held[i] || (j < s.pages[i] && e.was == e.is) || checked_page(e.was, a.num_pages) < 0) return false;
-  return __hip_atomic_load(a.marks + e.was, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-         (call << 16 | static_cast<uint32_t>(i + 1));
+  return __hip_atomic_load(a.marks + e.was, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == mark;
 }
+__device__ __forceinline__ uint64_t row_mark(uint64_t call, int row) { return call << 16 | static_cast<uint32_t>(row + 1) << 1; }
 
 // Small tables: one block does everything, a chain of reads and barriers. (4 rows of 70 pages 7 us, 16 of 64 8.5, 64 of 64 19.4; the
 // three launches below 11.4, 11.7 and 12.6 of kernel time: each 1024 entries take the block two turns, 3.6 us.)
@@ -207,9 +209,10 @@ __global__ __launch_bounds__(kSmallThreads) void k_fork_small(ForkArgs a) {
   const int wide = s.wide, entries = a.n * wide;
   const uint64_t call = status == 0 ? number : 0;
   bool any = false;
+  uint64_t before;
   for (int e = tid; e < entries; e += kSmallThreads) {
     const int i = e / wide, j = e - i * wide;
-    any |= fork_mark(a, s, i, j, fork_entry(a, s, i, j, head0), call);
+    any |= fork_mark(a, s, i, j, fork_entry(a, s, i, j, head0), call, call << 16 | static_cast<uint32_t>(e + 1), &before);
   }
   int64_t back = 0;  // pages given back so far
   if (__syncthreads_or(any)) {
@@ -217,7 +220,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_fork_small(ForkArgs a) {
     for (int e0 = 0, turn = 0; e0 < entries; e0 += kSmallThreads, turn ^= 1) {
       const int e = e0 + tid, i = min(e, entries - 1) / wide, j = min(e, entries - 1) - i * wide;
       const ForkEntry entry = fork_entry(a, s, i, j, head0);
-      const bool free = e < entries && fork_frees(a, s, i, j, entry, call);
+      const bool free = e < entries && fork_frees(a, s, i, j, entry, call << 16 | static_cast<uint32_t>(e + 1));
       const uint64_t wave = __ballot(free);
       if (lane == 0) freed[turn][wid] = __popcll(wave);
       __syncthreads();
@@ -252,7 +255,12 @@ __global__ __launch_bounds__(kSmallThreads) void k_fork_mark(ForkArgs a) {
   constexpr int kUnits = kSmallThreads / kForkThreads;  // of a block at a time
   for (int u = blockIdx.x * kUnits + threadIdx.x / kForkThreads; u < a.n * a.chunks; u += gridDim.x * kUnits) {
     const int i = u / a.chunks, j = (u - i * a.chunks) * kForkThreads + threadIdx.x % kForkThreads;
-    if (j < max(s.held[i], s.pages[i])) fork_mark(a, s, i, j, fork_entry(a, s, i, j, head0), call);
+    if (j >= max(s.held[i], s.pages[i])) continue;
+    const ForkEntry e = fork_entry(a, s, i, j, head0);
+    const uint64_t mark = row_mark(call, i);
+    uint64_t before;
+    if (fork_mark(a, s, i, j, e, call, mark, &before) && (before | 1) == (mark | 1))
+      atomicMax(reinterpret_cast<unsigned long long*>(a.marks + e.was), static_cast<unsigned long long>(mark | 1));
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.found[0] = head;
@@ -275,8 +283,12 @@ __global__ __launch_bounds__(kForkThreads) void k_fork_find(ForkArgs a) {
     int32_t was = -1;
     if (j < held) {
       was = a.table[i * a.table_stride + j];
-      if (checked_page(was, a.num_pages) >= 0 && (j >= pages || a.new_table[i * a.table_stride + j] != was))
-        free = a.marks[was] == (call << 16 | static_cast<uint32_t>(i + 1));
+      if (checked_page(was, a.num_pages) >= 0 && (j >= pages || a.new_table[i * a.table_stride + j] != was)) {
+        const uint64_t word = a.marks[was], mark = row_mark(call, i);
+        free = (word | 1) == (mark | 1);
+        if (free && word != mark)
+          for (int k = j + 1; k < held && free; ++k) free = a.table[i * a.table_stride + k] != was;
+      }
     }
     const uint64_t wave = __ballot(free);
     if (lane == 0) freed[turn][wid] = __popcll(wave);

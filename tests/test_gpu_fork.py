@@ -261,6 +261,38 @@ def test_fork_with_foreign_page_ids(gpu_ctx, n, width):
     check_fork(gpu_ctx, parents, None, old, 16, table, ring, cursors)
 
 
+@pytest.mark.parametrize("n,width", [(3, 12), (5, 400), (3, 9000), (1030, 70)])
+def test_fork_frees_a_page_once_that_a_row_names_twice(gpu_ctx, n, width):
+    """A table that no plan or fork makes: a row with the same page at several places. It goes to the ring once, in the place of
+    the last of them, wherever they lie; and not at all where one of them goes on."""
+    rng = np.random.default_rng(width)
+    page, long = 16, min(width, 5000)
+    old = np.minimum(rng.integers(1, 6 * page, n), width * page)
+    old[:3] = long * page - 3
+    used = -(-old // page)
+    num_pages = int(used.sum()) + 3 * n
+    order = rng.permutation(num_pages).astype(np.int32)
+    table, at = np.full((n, width), -1, np.int32), 0
+    for i in range(n):
+        table[i, : used[i]] = order[at: at + used[i]]
+        at += used[i]
+    free = order[at:]
+    ring = np.full(num_pages, -7, np.int32)
+    ring[: free.size] = free
+    table[0, long - 1] = table[0, 0]                                     # the ends of a row
+    table[0, 1: long - 1: 3] = table[0, 2]                               # many times
+    table[1, rng.integers(0, long, long // 2)] = table[1, long // 2]     # and in two rows
+    table[2, rng.integers(0, long, 4)] = table[1, long // 2]
+    cursors = [0, free.size]
+    for parents in ([-1, -1, -1], [0, 0, -1], [-1, 2, 1], [1, -1, 2]):
+        parents = np.concatenate([parents, np.where(rng.random(n - 3) < 0.5, np.arange(3, n), -1)]).astype(np.int64)
+        keep = np.where(parents >= 0, old[np.maximum(parents, 0)], 0)
+        want = check_fork(gpu_ctx, parents, keep, old, page, table, ring, cursors)
+        entries = want[1][np.arange(want[2][0], want[2][1]) % num_pages]
+        assert len(set(entries.tolist())) == entries.size
+        check_fork(gpu_ctx, parents, np.minimum(keep, page * (long // 2)), old, page, table, ring, cursors)
+
+
 def test_fork_of_two_pools_in_turn(gpu_ctx):
     """Calls of one context on pools of different sizes, the second growing what the context keeps for each page."""
     rng = np.random.default_rng(9)
