@@ -332,9 +332,11 @@ template <int N>
 __device__ __forceinline__ void wait_loads() {
   __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
 }
-// A barrier with no fence: loads into LDS stay on their way across it.
+// A barrier with no fence: loads into LDS stay on their way across it. This wave's reads of LDS are over before it (nothing else
+// makes them: their results may be used behind the barrier, when other waves' loads already take the place).
 __device__ __forceinline__ void block_barrier() {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0) alone
   __builtin_amdgcn_s_barrier();
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
