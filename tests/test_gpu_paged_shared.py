@@ -436,3 +436,32 @@ def test_a_row_s_bits_at_the_edge_of_a_rescale(gpu_ctx, rows, nkv, prefix, secon
     q[1:, :, 2] = 1
     two = b.run(gpu_ctx, dtype, q=q.reshape(rows, -1), scale=unit_scale())
     assert np.array_equal(one[0][0], two[0][0]) and np.array_equal(one[1][0], two[1][0])
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("nq", [8, 24])
+def test_wrong_hints_about_prefixes_that_are_read_once(gpu_ctx, page, nq):
+    """Prefixes of 256 keys and more, which are read once (shorter ones are each row's own keys): starts out of order or out of
+    range, prefixes that are cut, negative or longer than the rows, bounds that are too low."""
+    sizes, prefix = [5, 1, 6], [400, 290, 333]
+    b = Batch(sizes, prefix, [3, 0, 10, 70, 31, 5, 1, 2, 3, 4, 5, 0], nq, 2, 128, page)
+    for kw in [{"starts": [0, 7, 3, 12]}, {"starts": [0, 5, 6, 13]}, {"starts": [1, 4, 6, 9], "prefix": [400, 0, 333]},
+               {"starts": [0, 0, 0, 5, 5, 6, 12, 12], "prefix": [9, 999, 400, 5, 290, 333, -4]}, {"starts": [6, 12], "prefix": [333]},
+               {"starts": [2, 5], "prefix": [300]}, {"prefix": [-1, -2 ** 31, 333]}, {"prefix": [399, 289, 256]},
+               {"prefix": [2 ** 31 - 1, 290, 333], "max_prefix": 400}, {"max_prefix": 255}, {"max_prefix": 256}, {"max_prefix": 287},
+               {"max_prefix": 300}, {"max_group": 2}, {"max_group": 5}, {"max_group": 4, "max_prefix": 320}]:
+        b.check(gpu_ctx, **kw)
+
+
+@pytest.mark.parametrize("nq", [8, 24])
+def test_a_prefix_longer_than_what_the_rows_share(gpu_ctx, nq):
+    """The caller's word, broken for the second group's rows, which share 290 positions and are said to share 384: one of them that
+    holds them all lends its pages to the others. The other groups' rows are as they were, and so are rows too short for it."""
+    b = Batch([3, 4, 2], [400, 290, 300], [3, 0, 10, 200, 150, 93, 120, 5, 6], nq, 2, 64, 16)
+    out, lse, q = b.run(gpu_ctx, prefix=[400, 384, 300], max_prefix=400)
+    for r in range(b.n):
+        k, v = b.rows[r]
+        if r in (4, 6):  # the first 384 positions are those of row 3, the first that holds them
+            k, v = (np.concatenate([lent[:, :384], own[:, 384:]], 1) for lent, own in zip(b.rows[3], b.rows[r]))
+        want, want_lse, tol, tol_lse = formula(q[r], k, v, 0.125)
+        assert (np.abs(out[r] - want) <= tol).all() and (np.abs(lse[r] - want_lse) <= tol_lse).all(), r
