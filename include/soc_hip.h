@@ -435,12 +435,15 @@ int soc_logprobs(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row_st
  *      of parents), soc_paged_fork (the table rows that follow the choice), soc_paged_copy (the pages that two rows would
  *      otherwise write, all layers), then a step as above from the lengths that the fork gives, its attention by
  *      soc_paged_attention_shared. Rows that share pages end, or get shorter than what they share, by a fork and not by a
- *      plan (which gives back each row's pages, whoever else names them). What holds for the calls above holds here. ---- */
+ *      plan (which gives back each row's pages, whoever else names them). What holds for the calls above holds here. What the
+ *      host plans by is max_pages, not the lengths: it is best no wider than the longest row needs, whatever table_stride is. ---- */
 /* The best continuations of `groups` requests with `beams` (1 to 64) beams each, at most 2^20 rows of logits (row g * beams +
  * b; `vocab` logits of SOC_DTYPE_F32 or _F16, at most 2^20, row_stride elements apart): the score of token v behind row r is
  * scores[r] + the log probability of v under softmax(row r / temperature) (temperature <= 0 taken as 1; at most 2^100). The
  * order of a request's continuations is by score, greater first; equal scores by lowest row, then as in soc_logprobs (by
- * logit, then lowest id). Scores are formed and compared in 64 bits and rounded to fp32 once.
+ * logit, then lowest id). Scores are formed and compared in 64 bits and rounded to fp32 once; the exponentials under the
+ * logarithm are fp32 ones, added in 64 bits from 8192 or 16384 on, by which the scores of a row are off by 5e-6 at most, all
+ * alike (continuations of different rows that are closer may stand the other way round; equal rows have equal scores).
  *   top_rows, top_tokens, top_scores [groups][top_n] (0 <= top_n <= 64; NULL at 0): the first top_n.
  *   next_rows, next_tokens, next_scores [groups * beams] (all or none NULL): each request's first `beams` whose token is none
  *     of stop_tokens [num_stops] (host memory; at most 8, and beams * (1 + num_stops) at most 64): its next beams, of which
@@ -460,7 +463,7 @@ int soc_beam_select(soc_ctx* ctx, const void* logits, int32_t dtype, int64_t row
  *   copies [n][3], of which *copy_count are written: (the page copied from, to, positions), as soc_paged_copy takes them.
  *     Entries behind them are left as they are.
  *   Pages that a row of block_table names within old_lens, and no row of new_table, go to the ring's tail, once each: rows in
- *     order, pages in order, each page in the place of the last row that lost it.
+ *     order, pages in order, each page in the last place that lost it.
  *   new_lens [n]: keep, or 0 where parents[i] is -1. next_lens [n] (nullable): one more where the row goes on, else 0 (what a
  *     plan takes as new_lens in a step of single tokens).
  * new_table must not overlap block_table (entries behind a row's pages are left as they are), new_lens and next_lens not
@@ -498,7 +501,8 @@ int soc_paged_compact(soc_ctx* ctx, int32_t n, const int32_t* lens, int32_t page
  * - 1 (device memory, groups + 1 entries, ascending; rows of no group stand for themselves), and the first prefix_lens[g]
  * positions of its rows hold the same keys and values, as a rule because they name the same pages. Those positions may be
  * read once for all the group's rows, from any of their pages; the rest from each row's own. That they are the same is the
- * caller's word. For the rest the groups are a hint: starts that do not ascend within the n rows, prefixes that are negative,
+ * caller's word: a prefix that is longer than what the rows share, but no longer than the rows, gives them one another's keys,
+ * with no sign of it. For the rest the groups are a hint: starts that do not ascend within the n rows, prefixes that are negative,
  * longer than a row or than max_prefix, rows beyond max_group in a group, prefixes too short to be worth it: then a row's
  * keys are read from its own pages. 1 <= groups <= 4096, no more than n. max_group (at least 1) and max_prefix (at least 0)
  * bound what is launched; bounds that ask for more than 2^23 blocks (a block: 64 columns of max_group * q_heads / kv_heads

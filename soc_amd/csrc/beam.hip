@@ -2,9 +2,9 @@
 // from one row (Mac/gpu/src/runtime/sampler.cpp:14-71).
 //
 // score(b, v) = cum_b + (x_bv - M_b) / t - log S_b, with M_b the row's largest logit and S_b = sum exp((x_bv - M_b) / t).
-// The terms of S are fp32 exponentials added in fp32 within a chunk; chunks are joined and scores formed in 64 bits, so that
-// beams of nearly the same score keep their order. A row's bits follow from its logits alone, not from where they lie:
-// equal beams have equal scores.
+// The terms of S are fp32 exponentials added in fp32 within a chunk; chunks are joined and scores formed in 64 bits: scores of a row
+// are off by 5e-6 at most, all alike, so that they keep their order however near they are. A row's bits follow from its
+// logits alone, not from where they lie: equal beams have equal scores.
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -85,7 +85,7 @@ __device__ __forceinline__ double score_value(uint64_t o) {
 // threads. A thread holds E logits v, logit e of id place(e) (of another thread: place_of(thread, e)), its largest `best`;
 // ids outside [0, vocab) are no tokens and their logits -inf. keys: n * E words of LDS. Each thread's largest token stands
 // for its E: the n-th largest of those keys is a threshold that at most n threads reach, so at most n E tokens (64 of
-// normal data) are candidates, and those rank each other. No step depends on how many values are equal. nans: whether a NaN
+// normal data) are candidates, and those rank each other. No step here depends on how many values are equal. nans: whether a NaN
 // may be among the logits. The rest is LDS; found and givers are 0 before the call, with a barrier since. (soc_logprobs has
 // these steps in its kernel: calling this takes it 0.3 us of 11 for one row.)
 template <typename T, int E, typename Place, typename PlaceOf>

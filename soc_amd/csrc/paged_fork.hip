@@ -362,8 +362,8 @@ struct CopyArgs {
 constexpr int kCopyEach = 8;  // vectors a thread has on their way
 
 // A unit is 2048 vectors of one page of one plane. Of a partly filled page the places in use are copied, head by head. Bound by
-// memory: 90 pages of 28 layers, 189 MB in all, 41 us, 4.6 TB/s, the rate of a large copy. Up to 64 layers a launch, whose planes are
-// kernel arguments: 3 partly filled pages take 4.3 us of the call's 8.
+// memory: 90 pages of 64 positions in 4 layers, 8 heads of 128, 189 MB in all, 41 us, 4.6 TB/s, the rate of a large copy. Up to 64
+// layers a launch, whose planes are kernel arguments: 3 partly filled pages of 28 layers take 4.3 us of the call's 8.
 __global__ __launch_bounds__(256) void k_paged_copy(CopyArgs a) {
   const int count = min(max(a.count != nullptr ? *a.count : a.room, 0), a.room);
   const int per_move = 2 * a.layers * a.parts;

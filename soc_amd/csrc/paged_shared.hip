@@ -8,9 +8,10 @@
 // head). (Joined by the last block to add one, a prefix's blocks have up to 16 of them to join one after the other: 16 groups
 // of 4 rows, 2000 common keys, took 100 us for 34.) Two ways to a part:
 //   a row's own keys, and up to 16 columns of a prefix: four waves take the 32-key tiles of a chunk in turn, all with the same
-//   columns, and add up their sums in LDS (24 groups of 1 to 8 rows with 4 heads each, fp16, 67 us; all in blocks of 64 columns 76);
+//   columns, and add up their sums in LDS (16 groups of 4 rows with 4 heads each behind 2000 common keys 36.5 us, all in blocks of
+//   64 columns 45.7; 24 groups of 1 to 8 rows in fp16 67 and 66);
 //   up to 64 columns of a prefix: four waves with 16 columns each, whose key tiles go through LDS (256 rows behind 4096 common keys
-//   146 us, with the first way alone 190).
+//   133 us, with the first way alone 194).
 // Keys and values are matrix operands as they come from memory:
 //   scores  S [16 keys][16 columns] = K . Q^T, v_mfma_f32_16x16x32_f16: lane l holds 8 dims of key l % 16, and of column
 //           l % 16. An fp32 query is an fp16 high part and what fp32 has beyond it, both added into one sum.
@@ -20,9 +21,9 @@
 // rescaled, and no maximum is sought otherwise. l is another row of O^T, of values 1.
 //
 // Bound: reading keys and values once. 256 rows behind 4096 common keys with 512 of their own, 32 query and 8 KV heads of 128,
-// fp32: 130 us, of which 122 reading 589 MB (4.8 TB/s; a large copy reaches 4.7); read row by row they would be 4.8 GB.
-// 24 groups of ragged rows in fp16, 259 MB: 66.7 us, 4.4 TB/s and 6 us of joining. The products of a prefix take 8.7 us per 1000
-// keys of those 256 rows, 0.97 PFLOP/s with both parts (a large fp16 product reaches 1.2): more than its reading beyond 64 rows.
+// fp32: 133 us, of which 123 reading 588 MB (4.8 TB/s; a large copy reaches 4.7); read row by row they would be 4.8 GB.
+// 24 groups of ragged rows in fp16, 260 MB: 67 us, 4.4 TB/s and 7 us of joining. The products of a prefix take 8.8 us per 1000
+// keys of those 256 rows, 0.96 PFLOP/s with both parts (a large fp16 product reaches 1.2): more than its reading beyond 64 rows.
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
@@ -39,8 +40,9 @@ namespace {
 constexpr int kTile = 32;  // keys of a step
 constexpr int kFew = 16, kMany = 64;  // columns of a block that takes a prefix
 constexpr int kMaxParts = 64;  // of a prefix, and of a row's own keys
-// A prefix worth a part of its own: 64 groups of 8 rows, 130 keys of their own, take 94 us for 104 where 256 are common, with 128
-// common ones 92 for 82; 128 groups of 2 rows, 300 of their own, 88 for 85 with 256, 64 of them with 512 and 100 43 for 45.
+// A prefix worth a part of its own: 64 groups of 8 rows, 130 keys of their own, take 96 us for 106 row by row where 256 are common,
+// with 128 common ones 92 for 84; 128 groups of 2 rows, 300 of their own, 96 for 87 with 256 and 82 for 72 with 128, 64 of them
+// with 512 and 100 49 for 46.
 constexpr int kShortest = 8 * kTile;
 
 struct SharedArgs {
@@ -217,7 +219,7 @@ __device__ __forceinline__ f16x8 all_ones() {
 }
 
 // One wave of four, 16 columns, every fourth tile; kOnce: keys that nobody else reads, past the caches (256 rows behind 4096
-// common keys 139 us, else 142). Keys and values go from memory to registers, 16 bytes a lane, the next tile's on their way; of
+// common keys 133 us, else 143). Keys and values go from memory to registers, 16 bytes a lane, the next tile's on their way; of
 // the 8 dims x 8 keys of values that a lane reads, v_perm_b32 makes the operand V^T, in whose rows dim d * 16 + i stands for
 // dim i * (HD / 16) + d. Whether a page was none of the cache.
 template <typename T, int HD, bool kOnce>
@@ -309,7 +311,8 @@ __device__ __forceinline__ bool attend_wave(const SharedArgs& a, int g, const Co
 }
 
 // A block's four waves, 16 columns each: the keys' tiles, which are whole, go through a ring in LDS, the next two on their way
-// while one is in use. A tile row's 16-byte chunk c lies at slot c ^ swizzle(row), so that 16 rows read at one chunk
+// while one's scores are formed. (Before a tile's transposing reads the compiler waits for all of them: it cannot tell the places
+// that they go to from those that are read.) A tile row's 16-byte chunk c lies at slot c ^ swizzle(row), so that 16 rows read at one chunk
 // reach all banks; ds_read_b64_tr_b16 gives V^T (in each 16-lane group, lane j names 4 dims of one key, and lane i receives
 // dim i of 4 keys).
 constexpr int kRing = 3;  // tiles in LDS
@@ -570,8 +573,8 @@ __device__ __forceinline__ void prefix_part(const SharedArgs& a, int unit, char*
     const int c = wid * 16 + (lane & 15), at = cols.first + c, r = at / G, h = at - r * G, row = lane >> 4;
     if (c >= cols.count || !holds(r)) return;
     float* part = part_of(r);
-    // past the caches, where the many parts of a block would push out what others read (256 rows behind 4096 common keys 130 us,
-    // with plain stores 138; the parts of the other way, fewer, gain nothing so)
+    // past the caches, where the many parts of a block would push out what others read (256 rows behind 4096 common keys 133 us,
+    // with plain stores 140, with no keys of their own 66 and 64; the parts of the other way, fewer, gain nothing so)
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d)
       __builtin_nontemporal_store(static_cast<Four>(sums.o[d]), reinterpret_cast<Four*>(part + h * HD + d * 16 + row * 4));
@@ -802,8 +805,8 @@ int soc_paged_attention_shared(soc_ctx* ctx, const soc_paged_cache* cache, const
   a.wide_q = reinterpret_cast<uintptr_t>(q) % (8 * size) == 0 && q_stride % 8 == 0;
   const int64_t longest = static_cast<int64_t>(max_pages) * cache->page_size;
   // Where there is nothing to share, or little to read, each row's keys are read for it alone, in one launch: 4 rows of 1100
-  // keys, 16 query and 8 KV heads (18 MB), 9.8 us so and 11.4 shared; 4 of 4100, 32 and 8 heads (67 MB) 14.7 both ways; 8 of 4160
-  // (136 MB) 20.5 and 15.0.
+  // keys, 16 query and 8 KV heads (18 MB), 9.9 us so and 11.8 shared; 4 of 4100, 32 and 8 heads (67 MB) 15.7 and 16.2; 8 of 4160
+  // (136 MB) 22.7 and 16.7. The table's width stands for the rows' lengths, which the host does not know.
   const int64_t bytes = pairs * longest * hd * 4;
   const char* always = std::getenv("SOC_PAGED_SHARED");  // =always: the tests' small sizes too
   const bool little = bytes < (int64_t{64} << 20) && !(always != nullptr && std::strcmp(always, "always") == 0);
@@ -818,15 +821,15 @@ int soc_paged_attention_shared(soc_ctx* ctx, const soc_paged_cache* cache, const
   a.columns = columns <= soc::kFew ? soc::kFew : soc::kMany;
   a.tiles = static_cast<int>((columns + a.columns - 1) / a.columns);
   const int64_t units = static_cast<int64_t>(groups) * a.nkv * a.tiles;
-  // a block for each CU where there are few (parts cost: 256 rows behind 4096 common keys, 512 of their own: 138 us, with twice
-  // as many blocks 156), and 1024 keys a block where there are many
+  // a block for each CU where there are few (parts cost: 64 rows behind 4096 common keys 26.0 us, with twice as many blocks 27.7; 16
+  // groups of 4 rows behind 2000 36.5 and 38.6), and 1024 keys a block where there are many
   a.prefix_chunks = soc::chunks_for(units, max_prefix, 256, 128, 1024, room);
   if (units * a.prefix_chunks.grid > (1 << 23))
     return soc::fail(SOC_ERR_INVALID, "shared attention: too many groups of this size");
   a.prefix_blocks = static_cast<int>(units * a.prefix_chunks.grid);
   a.own_chunks = soc::chunks_for(pairs, longest, 256, 128, 1024, room);
   // what a row has behind the longest prefix: no more blocks are launched for a row than twice that takes, or 1024 for all rows
-  // (256 rows behind 12000 common keys, 10 of their own: 129 us, with eight blocks a row 150). A row that shares nothing has
+  // (256 rows behind 12000 common keys, 10 of their own: 135 us, with eight blocks a row 172). A row that shares nothing has
   // few blocks then
   const int64_t own = std::max<int64_t>(1, longest - max_prefix);
   const int64_t few = std::max<int64_t>(2 * soc::chunks_for(pairs, own, 256, 128, 1024, room).grid, 1024 / pairs);

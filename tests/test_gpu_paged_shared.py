@@ -1,5 +1,7 @@
 """Attention of one token of each sequence where groups of sequences share a prefix (soc_paged_attention_shared) against the
-formula in 64 bits; the groups are a hint, so that wrong ones change nothing but the time.
+formula in 64 bits. That a group's rows share its prefix is the caller's word; the rest of the groups is a hint, so that
+malformed ones, and prefixes longer than rows, change nothing but the time. (Prefixes of less than 256 keys are each row's own
+keys, whatever the groups.)
 
 Tolerance. A score is a sum of 2 head_dim products (queries as two fp16 parts, exact to 2^-22), added in 32 bits in any order:
 off by (2 head_dim + 8) 2^-24 sum |q_i k_i| scale = e. A weight is then off by 2 e + 8 2^-24 relative, the weighted sum by
@@ -212,7 +214,7 @@ def test_wrong_hints_change_no_result(gpu_ctx, page):
                {"max_group": 1}, {"max_group": 2}, {"max_group": 4}, {"max_group": 12}, {"max_group": 5, "max_prefix": 200},
                {"max_group": 2 ** 31 - 1, "max_prefix": 2 ** 31 - 1}]:
         b.check(gpu_ctx, **kw)
-    # one more than the rows share: too long for a row without a tail, which reads its own keys; the others' word is broken
+    # prefixes as long as a number can be, cut to max_prefix; rows that end before it read their own keys; the last row in no group
     b.check(gpu_ctx, prefix=[2 ** 31 - 1, 130, 2 ** 31 - 1], max_prefix=333, starts=[0, 0, 5, 11])
 
 
